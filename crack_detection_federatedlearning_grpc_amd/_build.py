@@ -125,7 +125,10 @@ def _hip_inputs():
     binding = os.path.join(CSRC, "bindings.cpp")
     inc, libs, abi = _torch_flags()
     base = ["-O3", "-fPIC", "-std=c++17", f"--offload-arch={ARCH}", f"-I{CSRC}", f"-I{CSRC}/kernels",
-            "-Wno-unused-result", "-Wno-unused-command-line-argument", "-ffp-contract=fast"]
+            "-Wno-unused-result", "-Wno-unused-command-line-argument", "-ffp-contract=fast",
+            # no packed fp32 instructions (v_pk_fma_f32 and its like): some of their forms have given wrong results
+            # on this hardware now and then; the two-element vector code compiles to pairs of plain ones instead
+            "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     import torch
     # the key must not depend on where the tree or torch live (the snapshot runs from another path on the GPU
     # box): source bytes + path-free flags + torch version + arch
