@@ -2,7 +2,7 @@
 
 * ``_native``  host C++ (HDF5 writer/reader, contour geometry, image resize): g++ + pybind11, no GPU toolchain.
 * ``_C``       HIP/CDNA4 kernels for gfx950 (``csrc/kernels/*.hip``, torch-free translation units compiled with
-               ``hipcc --offload-arch=gfx950``) + one binding TU (``csrc/bindings.cpp``, torch/extension.h).
+               ``hipcc --offload-arch=gfx950``) + the binding TUs (``csrc/*.cpp``, torch/extension.h).
 
 Objects are cached under ``build/`` keyed by a hash of (source, headers, flags); the ``.so`` files land inside the
 package so they travel with the repo snapshot to the GPU box.
@@ -122,7 +122,7 @@ def _torch_flags():
 def _hip_inputs():
     kern = sorted(glob.glob(os.path.join(CSRC, "kernels", "*.hip")))
     headers = sorted(glob.glob(os.path.join(CSRC, "kernels", "*.h")) + glob.glob(os.path.join(CSRC, "*.h")))
-    binding = os.path.join(CSRC, "bindings.cpp")
+    bindings = sorted(glob.glob(os.path.join(CSRC, "*.cpp")))
     inc, libs, abi = _torch_flags()
     base = ["-O3", "-fPIC", "-std=c++17", f"--offload-arch={ARCH}", f"-I{CSRC}", f"-I{CSRC}/kernels",
             "-Wno-unused-result", "-Wno-unused-command-line-argument", "-ffp-contract=fast",
@@ -133,8 +133,8 @@ def _hip_inputs():
     # the key must not depend on where the tree or torch live (the snapshot runs from another path on the GPU
     # box): source bytes + path-free flags + torch version + arch
     portable = [f for f in base if not f.startswith("-I")] + [torch.__version__, ARCH, str(abi)]
-    key = _hash(kern + headers + [binding], portable)
-    return kern, headers, binding, inc, libs, abi, base, key
+    key = _hash(kern + headers + bindings, portable)
+    return kern, headers, bindings, inc, libs, abi, base, key
 
 
 def hip_key() -> str:
@@ -142,7 +142,7 @@ def hip_key() -> str:
 
 
 def build_hip(force: bool = False, verbose: bool = True, jobs: int = 0) -> str:
-    kern, headers, binding, inc, libs, abi, base, key = _hip_inputs()
+    kern, headers, bindings, inc, libs, abi, base, key = _hip_inputs()
     out = hip_path()
     stamp = out + ".stamp"
     if not force and is_current(out, key):
@@ -163,7 +163,7 @@ def build_hip(force: bool = False, verbose: bool = True, jobs: int = 0) -> str:
 
     bflags = inc + _pybind_includes() + [f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_C",
                                          "-DTORCH_API_INCLUDE_EXTENSION_H", "-x", "hip"]
-    js = [job(s, []) for s in kern] + [job(binding, bflags)]
+    js = [job(s, []) for s in kern] + [job(b, bflags) for b in bindings]
     objs = _compile_all(js, jobs or min(8, os.cpu_count() or 4))
     tmp = out + ".tmp"
     _run([HIPCC, "-shared", f"--offload-arch={ARCH}", "-o", tmp, *objs, *libs])

@@ -12,6 +12,13 @@ are bf16 (``torch.bfloat16``); weights are fp32 in the Keras layouts the referen
 
 Backward: data gradient with the dgrad-packed weights through the same forward kernels, weight gradient through
 conv_wgrad / conv3x3_wgrad / dw_wgrad (fp32 accumulation). Shapes the kernels do not cover raise.
+
+Layers of a transformer block over the same maps, their pixels read as tokens (B, H * W, heads, C // heads):
+
+    y = layer_norm(x, w, b)               # Keras LayerNormalization           (norm.py;      kernel: layer_norm.hip)
+    q = rotary(q, positions, dims)        # rotary positions, 1-4 axes         (rotary.py;    kernel: rotary.hip)
+    y = attention(q, k, v, ...)           # softmax(q k^T) v, masked / causal  (attention.py; kernel: attention*.hip)
+    y = self_attention2d(x, ...)          # the block of them with 1x1 convs   (block.py)
 """
 from __future__ import annotations
 
@@ -143,4 +150,10 @@ def depthwise3x3(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     return _Depthwise.apply(x, w)
 
 
-__all__ = ["conv2d", "conv2d_transpose", "depthwise3x3"]
+from .attention import attention, attention_qkv  # noqa: E402
+from .block import self_attention2d  # noqa: E402
+from .norm import layer_norm  # noqa: E402
+from .rotary import grid_positions, rotary  # noqa: E402
+
+__all__ = ["conv2d", "conv2d_transpose", "depthwise3x3", "attention", "attention_qkv", "grid_positions", "layer_norm",
+           "rotary", "self_attention2d"]

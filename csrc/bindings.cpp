@@ -8,6 +8,7 @@
 #include <string>
 #include <vector>
 
+#include "block_ops.h"
 #include "kernels/launch.h"
 
 namespace {
@@ -873,6 +874,7 @@ void gather_rows_u8_op(at::Tensor src, at::Tensor idx, at::Tensor dst, int64_t r
 }  // namespace
 
 PYBIND11_MODULE(_C, m) {
+  bind_block_ops(m);
   m.doc() = "CDNA4 (gfx950) HIP kernels of the crack-segmentation FL trainer";
   m.attr("STAT_REPLICAS") = STAT_REPLICAS;
   m.def("conv_igemm", &conv_igemm_op, py::arg("x"), py::arg("wt"), py::arg("bias"), py::arg("y"), py::arg("stats"),

@@ -1,0 +1,200 @@
+// Shared parts of the attention kernels (attention.hip: forward, attention_bwd.hip: backward).
+//
+// Rows. The queries of the G = Hq / Hkv heads that share a key head are packed into one row axis, row r = i * G + g
+// (query i, head hkv * G + g), M = Sq * G rows per (image, key head). One block then reads a key head once for all of
+// them, gradients of a shared head are plain sums over its rows, and a few queries still fill a tile.
+//
+// MFMA layouts (v_mfma_f32_32x32x16): lane l = (c = l % 32, h = l / 32).
+//   A operand: row c, reduction slots 8h + j       B operand: column c, reduction slots 8h + j       (j = 0..7)
+//   result:    column c, element e (0..15) is row rowof(e) = (e & 3) + 8 * (e >> 2) + 4 * h
+// Both products of a pair are arranged so that the first one's result IS the second one's B operand: elements
+// 8s .. 8s + 7 of a result are 16 of its 32 rows (16s + {0-3, 8-11} + 4h), so with the A operand's slots taken in the
+// same order (two transposing LDS reads of 4 rows each) no lane exchanges anything between the products.
+#pragma once
+#include "common.h"
+#include "launch.h"
+
+namespace attn {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+
+typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
+typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+
+struct BF16 {
+  static CFL_DEVICE f16v mma(const s8v& a, const s8v& b, const f16v& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8v, a), __builtin_bit_cast(bf8v, b), c, 0, 0,
+                                                   0);
+  }
+  static CFL_DEVICE uint32_t pack2(float a, float b) { return pack2bf(a, b); }
+  static CFL_DEVICE float lo(uint32_t w) { return __uint_as_float(w << 16); }
+  static CFL_DEVICE float hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+};
+
+struct FP16 {
+  static CFL_DEVICE f16v mma(const s8v& a, const s8v& b, const f16v& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
+  }
+  static CFL_DEVICE uint32_t pack2(float a, float b) {
+    const f32x2_t v = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, h2v));
+  }
+  static CFL_DEVICE float lo(uint32_t w) { return (float)__builtin_bit_cast(h2v, w)[0]; }
+  static CFL_DEVICE float hi(uint32_t w) { return (float)__builtin_bit_cast(h2v, w)[1]; }
+};
+
+CFL_DEVICE int rowof(int e, int h) { return (e & 3) + 8 * (e >> 2) + 4 * h; }
+
+CFL_DEVICE float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// value of the lane 32 away
+CFL_DEVICE float other_half(float v) {
+  const unsigned u = __builtin_bit_cast(unsigned, v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_bit_cast(float, (threadIdx.x & 32) ? (unsigned)r[0] : (unsigned)r[1]);
+}
+
+// LDS image of a tile of token rows, DP 16-bit values each: row-major without padding (an LDS-DMA load writes 16
+// bytes a lane, lanes in order), the 16-byte chunks of a row permuted by its index. Eight rows in a row then hold a
+// given chunk in eight different 16-byte bank groups (fragment reads, ds_read_b128), and four rows in a row hold a
+// given 64-byte quarter alternately in both halves of the 128-byte bank line (transposing reads, ds_read_b64_tr_b16).
+template <int DP>
+CFL_DEVICE int swz(int row) {
+  if (DP % 64 != 0) return (row >> 1) & 3;             // rows of 64 or 192 bytes alternate the halves by themselves
+  return ((row & 1) << 2) | ((row >> 1) & 3);
+}
+template <int DP>
+CFL_DEVICE int lds_at(int row, int chunk) { return row * DP + ((chunk ^ swz<DP>(row)) << 3); }
+
+// A operand of a product that reduces over d: row `row`, chunk = 2 * kk + h
+template <int DP>
+CFL_DEVICE s8v frag(const bf16_t* tile, int row, int chunk) {
+  return *reinterpret_cast<const s8v*>(tile + lds_at<DP>(row, chunk));
+}
+
+CFL_DEVICE s4v tr4(const bf16_t* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4v __attribute__((address_space(3)))*)(p));
+}
+
+// A operand of a product that reduces over token rows: operand row = channel 32 * dt + c, slots = token rows
+// row0 + {0-3, 8-11} + 4h (row0 a multiple of 16)
+template <int DP>
+CFL_DEVICE s8v frag_t(const bf16_t* tile, int row0, int dt, int lane) {
+  const int p = lane & 15, row = row0 + ((lane >> 5) << 2) + (p >> 2);
+  const int col = 32 * dt + (lane & 16) + ((p & 3) << 2);
+  const s4v a = tr4(tile + lds_at<DP>(row, col >> 3) + (col & 7));
+  const s4v b = tr4(tile + lds_at<DP>(row + 8, col >> 3) + (col & 7));
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// eight elements 8s .. 8s + 7 of a result, rounded to 16 bits: the B operand of the second product
+template <class T>
+CFL_DEVICE s8v pack_b(const f16v& v, int s) {
+  const u4v w = {T::pack2(v[8 * s], v[8 * s + 1]), T::pack2(v[8 * s + 2], v[8 * s + 3]),
+                 T::pack2(v[8 * s + 4], v[8 * s + 5]), T::pack2(v[8 * s + 6], v[8 * s + 7])};
+  return __builtin_bit_cast(s8v, w);
+}
+
+// 32 channels 32 * dt .. + 31 of one token row per lane pair (c, c + 32): four quads each, exchanged between the
+// halves so that a lane stores 16 contiguous bytes (lane half h: channels 16s + 8h .. + 7)
+template <class T>
+CFL_DEVICE void store_row(bf16_t* row, const f16v& v, float mul, int dt, int D, int h, bool ok) {
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const unsigned a0 = T::pack2(v[8 * s] * mul, v[8 * s + 1] * mul);
+    const unsigned a1 = T::pack2(v[8 * s + 2] * mul, v[8 * s + 3] * mul);
+    const unsigned b0 = T::pack2(v[8 * s + 4] * mul, v[8 * s + 5] * mul);
+    const unsigned b1 = T::pack2(v[8 * s + 6] * mul, v[8 * s + 7] * mul);
+    const auto x = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
+    const auto y = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
+    const int d = 32 * dt + 16 * s + 8 * h;
+    if (ok && d < D) *reinterpret_cast<uint4*>(row + d) = make_uint4(x[0], y[0], x[1], y[1]);
+  }
+}
+
+// 16 bytes of the buffer at byte offset `off` -> LDS at the wave-uniform `lds` + 16 * lane; an offset past the range
+// writes zeros. Inline asm: with the builtin the compiler orders every later LDS read behind all loads in flight. The
+// caller waits with wait_vm() before the barrier that publishes the tile.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+CFL_DEVICE void dma16(const u4v& rs, uint32_t off, const bf16_t* lds) {
+  const uint32_t a =
+      __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(a), "v"(off), "s"(rs)
+               : "memory", "m0");
+}
+CFL_DEVICE void dma4(const u4v& rs, uint32_t off, const float* lds) {      // the same, 4 bytes a lane
+  const uint32_t a =
+      __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(a), "v"(off), "s"(rs)
+               : "memory", "m0");
+}
+#pragma clang diagnostic pop
+CFL_DEVICE void wait_vm() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+CFL_DEVICE u4v rsrc(const void* base) {
+  const uint64_t a = reinterpret_cast<uint64_t>(base);
+  u4v r;
+  r.x = __builtin_amdgcn_readfirstlane((int)(uint32_t)a);
+  r.y = __builtin_amdgcn_readfirstlane((int)((uint32_t)(a >> 32) & 0xffffu));
+  r.z = CFL_OOB - 1;
+  r.w = 0x00020000;
+  return r;
+}
+
+CFL_DEVICE int fdiv(int x, const FastDiv& f) { return fdiv32(x, f); }
+
+// Which tiles of a walk hold any allowed pair, and which only allowed ones, for the block: lanes look up the classes of
+// 64 tiles ahead at a time, two ballots keep them.
+struct TileMask {
+  unsigned long long live, whole;
+  int base;
+  int64_t lead0, leadg;          // class rows of this block's first head, and from one head to the next
+  int heads, nib;
+
+  CFL_DEVICE void init(const AttnParams& p, int b, int hk) {
+    nib = (p.mask.rows + 31) >> 5;
+    // sb / sh count mask rows, `rows` of them for each (image, head) entry
+    lead0 = (b * p.mask.sb + (int64_t)hk * p.G * p.mask.sh) / p.mask.rows;
+    leadg = p.mask.sh ? 1 : 0;
+    heads = p.mask.sh ? p.G : 1;
+    base = -64;
+    live = whole = 0;
+  }
+  // 0 / 1 / 2 as the mask's classes, over queries i0 .. i1 and words w0 .. w1 (this lane's tile; `in`: it exists)
+  CFL_DEVICE int cls(const AttnParams& p, int i0, int i1, int w0, int w1, bool in) const {
+    bool any = false, all = true;
+    if (in) {
+      const int b0 = p.mask.rows > 1 ? i0 >> 5 : 0, b1 = p.mask.rows > 1 ? i1 >> 5 : 0;
+      for (int g = 0; g < heads; ++g)
+        for (int ib = b0; ib <= b1; ++ib)
+          for (int w = w0; w <= w1; ++w) {
+            const int k = p.mask.cls[((lead0 + g * leadg) * nib + ib) * p.mask.words + w];
+            any |= k != 0;
+            all &= k == 2;
+          }
+    }
+    return any ? (all ? 2 : 1) : 0;
+  }
+  // first tile at or after t with an allowed pair, t1 if there is none before it
+  template <class F>
+  CFL_DEVICE int next(int t, int t1, const F& f) {
+    while (t < t1) {
+      if (t - base >= 64) {
+        const int k = f(t + (int)(threadIdx.x & 63));
+        live = __ballot(k != 0);
+        whole = __ballot(k == 2);
+        base = t;
+      }
+      const unsigned long long rest = live >> (t - base);
+      if (rest) return imin(t + __builtin_ctzll(rest), t1);
+      t = base + 64;
+    }
+    return t1;
+  }
+  CFL_DEVICE bool is_whole(int t) const { return (whole >> ((t - base) & 63)) & 1; }
+};
+
+}  // namespace attn

@@ -1,0 +1,428 @@
+// Attention, forward:  o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i.k_j - lse_i) over the keys j that row i may attend.
+//
+// One pass over the keys with the running maximum and sum of the softmax. S^T = K Q^T is computed instead of Q K^T, so a
+// lane holds 16 keys of ONE row (attention.h): the row's maximum and sum are sums within the lane plus one exchange with
+// the lane 32 away, the rescaling factor is the lane's own scalar, and exp(S^T) rounded to 16 bits is the B operand of
+// O^T = V^T P^T as it stands. K and V tiles go from memory to LDS by LDS-DMA loads, one tile ahead.
+//
+// Rounding: scores, maximum, sum and output accumulate in fp32. P is rounded to the inputs' type (relative error at most
+// half a step per term, independent from key to key), the output once.
+// Rows that may attend nothing are 0 and their saved lse2 is +inf (exp2(s - inf) = 0 in the backward pass).
+#include <algorithm>
+
+#include "attention.h"
+
+namespace {
+
+using namespace attn;
+
+// row maxima may lag the running maximum by 2^SLACK: P then reaches 2^SLACK (exact in both types' range, the relative
+// precision is the same) and most tiles rescale nothing
+constexpr float SLACK = 8.f;
+
+// QT: 32-row tiles per wave; WR x WK: waves along the rows and along the keys of a tile; KW keys per wave and tile
+template <class T, int DP, int QT, int WR, int WK, int KW, bool MASK>
+__global__ __launch_bounds__(64 * WR * WK) void attn_fwd_kernel(const AttnParams p) {
+  constexpr int NT = 64 * WR * WK, KT = KW * WK, TILE = KT * DP, CPR = DP / 8, CH = KT * CPR / NT;
+  constexpr int NK = KW / 32, NKK = DP / 16, ND = DP / 32;
+  static_assert(KT * CPR % NT == 0, "whole DMA instructions");
+  __shared__ __attribute__((aligned(1024))) bf16_t smem[4 * TILE];
+
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 31, h = lane >> 5, wr = wid / WK, wk = wid % WK;
+  constexpr int BR = 32 * QT * WR;
+  const int nrb = (p.M + BR - 1) / BR, bhn = p.B * p.Hkv;
+  const int lin = xcd_swizzle(blockIdx.x, gridDim.x);
+  const int rb0 = lin % nrb, rest = lin / nrb, bh = rest % bhn, sp = rest / bhn;
+  const int rb = p.causal ? nrb - 1 - rb0 : rb0;          // causal: long rows first
+  const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
+  const int len = p.lengths ? imin(imax(p.lengths[b], 0), p.Sk) : p.Sk;
+  const int off = p.causal ? p.Sk - p.Sq : 0;
+  const int r_end = imin(rb * BR + BR, p.M);
+
+  // this lane's rows: their queries as B operands, and the first key each may not attend
+  s8v qf[QT][NKK];
+  int lim[QT], ri[QT], rg[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = rb * BR + (wr * QT + t) * 32 + c;
+    const bool ok = r < p.M;
+    const int rr = ok ? r : p.M - 1, i = fdiv(rr, p.div_g), g = rr - i * p.G;
+    ri[t] = i;
+    rg[t] = g;
+    lim[t] = !ok ? 0 : p.causal ? imin(imax(i + off + 1, 0), len) : len;
+    const bf16_t* q = reinterpret_cast<const bf16_t*>(p.q.p) + b * p.q.sb + i * p.q.ss + (hk * p.G + g) * p.q.sh;
+#pragma unroll
+    for (int kk = 0; kk < NKK; ++kk) {
+      const int d = 16 * kk + 8 * h;
+      u4v w = {0, 0, 0, 0};
+      if (ok && d < p.D) w = *reinterpret_cast<const u4v*>(q + d);
+      qf[t][kk] = __builtin_bit_cast(s8v, w);
+    }
+  }
+  // first key past every row of the block / of this wave (rows are in query order)
+  const int i_last = fdiv(r_end - 1, p.div_g);
+  const int kend = p.causal ? imin(imax(i_last + off + 1, 0), len) : len;
+  const int wr0 = rb * BR + wr * QT * 32;
+  const int wi0 = fdiv(imin(wr0, p.M - 1), p.div_g), wi1 = fdiv(imin(wr0 + QT * 32, p.M) - 1, p.div_g);
+  const int wlast = wr0 >= p.M ? 0 : p.causal ? imin(imax(wi1 + off + 1, 0), len) : len;
+  const int wfull = p.causal ? imin(imax(wi0 + off + 1, 0), len) : len;   // keys below it: allowed for every row
+
+  const int tiles = (p.Sk + KT - 1) / KT, tps = (tiles + p.splits - 1) / p.splits;
+  const int t0 = sp * tps, t1 = imin(imin(t0 + tps, tiles), (kend + KT - 1) / KT);
+
+  // the block's part of a tile: CH 16-byte chunks per thread and tensor, the swizzle in the source address
+  uint32_t vk[CH], vv[CH];
+  int vrow[CH];
+#pragma unroll
+  for (int n = 0; n < CH; ++n) {
+    const int id = tid + NT * n, row = id / CPR, d = ((id % CPR) ^ swz<DP>(row)) * 8;
+    vrow[n] = d < p.D ? row : 0x7fffffff;
+    vk[n] = (uint32_t)(row * (int)p.k.ss + d) * 2;
+    vv[n] = (uint32_t)(row * (int)p.v.ss + d) * 2;
+  }
+  const bf16_t* kb = reinterpret_cast<const bf16_t*>(p.k.p) + b * p.k.sb + hk * p.k.sh;
+  const bf16_t* vb = reinterpret_cast<const bf16_t*>(p.v.p) + b * p.v.sb + hk * p.v.sh;
+  auto issue = [&](int t, int buf) {
+    const int rem = len - t * KT;
+    const u4v rk = rsrc(kb + (int64_t)t * KT * p.k.ss), rv = rsrc(vb + (int64_t)t * KT * p.v.ss);
+    const bf16_t* dst = smem + buf * 2 * TILE + wid * 512;
+#pragma unroll
+    for (int n = 0; n < CH; ++n) {
+      dma16(rk, vrow[n] < rem ? vk[n] : CFL_OOB, dst + NT * 8 * n);
+      dma16(rv, vrow[n] < rem ? vv[n] : CFL_OOB, dst + TILE + NT * 8 * n);
+    }
+  };
+
+  // boolean mask: this lane's rows' words
+  const unsigned long long* mrow[QT];
+  unsigned long long word[QT];
+  if (MASK) {
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+      mrow[t] = p.mask.bits + (b * p.mask.sb + (hk * p.G + rg[t]) * p.mask.sh + (p.mask.rows > 1 ? ri[t] : 0)) *
+                                  (int64_t)p.mask.words;
+  }
+  TileMask tm;
+  if (MASK) tm.init(p, b, hk);
+  const int i_first = fdiv(rb * BR, p.div_g);
+  auto next = [&](int t) {
+    if (!MASK) return t;
+    return tm.next(t, t1, [&](int u) {
+      return tm.cls(p, i_first, i_last, u * KT / 64, imin((u * KT + KT - 1) / 64, p.mask.words - 1), u < tiles);
+    });
+  };
+  auto words = [&](int t) {
+    const int w = imin((t * KT + wk * KW) >> 6, p.mask.words - 1);
+#pragma unroll
+    for (int u = 0; u < QT; ++u) word[u] = mrow[u][w];
+  };
+
+  f16v acc[ND][QT];
+  float m[QT], l[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    m[t] = -INFINITY;
+    l[t] = 0.f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[d][t][e] = 0.f;
+  }
+  const float sc = p.scale * LOG2E;
+
+  int t = next(t0), buf = 0;
+  if (t < t1) {
+    if (MASK) words(t);
+    issue(t, 0);
+  }
+  wait_vm();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  while (t < t1) {
+    const bool part = MASK && !tm.is_whole(t);
+    const int tn = next(t + 1);
+    unsigned long long cur[QT];
+    const int key0 = t * KT + wk * KW;
+    if (MASK) {
+#pragma unroll
+      for (int u = 0; u < QT; ++u) cur[u] = word[u] >> (key0 & 32);
+      if (tn < t1) words(tn);
+    }
+    if (tn < t1) issue(tn, buf ^ 1);
+
+    if (key0 < wlast) {
+      const bf16_t* sk = smem + buf * 2 * TILE + wk * KW * DP;
+      const bf16_t* sv = sk + TILE;
+      f16v s[NK][QT];
+#pragma unroll
+      for (int k = 0; k < NK; ++k)
+#pragma unroll
+        for (int u = 0; u < QT; ++u)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[k][u][e] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < NKK; ++kk)
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+          const s8v a = frag<DP>(sk, 32 * k + c, 2 * kk + h);
+#pragma unroll
+          for (int u = 0; u < QT; ++u) s[k][u] = T::mma(a, qf[u][kk], s[k][u]);
+        }
+      if (MASK && part) {
+#pragma unroll
+        for (int u = 0; u < QT; ++u)
+#pragma unroll
+          for (int k = 0; k < NK; ++k) {
+            const uint32_t w = (uint32_t)(cur[u] >> (32 * k)) >> (4 * h);
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              s[k][u][e] = (w >> ((e & 3) + 8 * (e >> 2))) & 1 ? s[k][u][e] : -INFINITY;
+          }
+      }
+      if (key0 + KW > wfull) {
+#pragma unroll
+        for (int u = 0; u < QT; ++u)
+#pragma unroll
+          for (int k = 0; k < NK; ++k) {
+            const int left = lim[u] - key0 - 32 * k - 4 * h;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[k][u][e] = (e & 3) + 8 * (e >> 2) < left ? s[k][u][e] : -INFINITY;
+          }
+      }
+      s8v pb[QT][2 * NK];
+#pragma unroll
+      for (int u = 0; u < QT; ++u) {
+        float mx = s[0][u][0];
+#pragma unroll
+        for (int k = 0; k < NK; ++k)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[k][u][e]);
+        mx = fmaxf(mx, other_half(mx)) * sc;
+        if (__any(mx > m[u] + SLACK)) {
+          const float mn = fmaxf(m[u], mx), al = exp2_(m[u] - (mn == -INFINITY ? 0.f : mn));
+          m[u] = mn;
+          l[u] *= al;
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[d][u][e] *= al;
+        }
+        const float ms = m[u] == -INFINITY ? 0.f : m[u];
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            s[k][u][e] = exp2_(fmaf(s[k][u][e], sc, -ms));
+            sum += s[k][u][e];
+          }
+          pb[u][2 * k] = pack_b<T>(s[k][u], 0);
+          pb[u][2 * k + 1] = pack_b<T>(s[k][u], 1);
+        }
+        l[u] += sum;
+      }
+#pragma unroll
+      for (int ks = 0; ks < 2 * NK; ++ks)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          const s8v a = frag_t<DP>(sv, 16 * ks, d, lane);
+#pragma unroll
+          for (int u = 0; u < QT; ++u) acc[d][u] = T::mma(a, pb[u][ks], acc[d][u]);
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    buf ^= 1;
+    t = tn;
+  }
+
+#pragma unroll
+  for (int u = 0; u < QT; ++u) l[u] += other_half(l[u]);
+
+  if constexpr (WK > 1) {
+    // join the waves that share rows: every wave's (m, l) and accumulators through LDS, wave w finishes the channel
+    // tiles w, w + WK, ...
+    static_assert(QT == 1 && WR == 1, "key-split waves hold one row tile");
+    constexpr int SEG = ND * 1024 + 128;                   // floats per wave
+      static_assert(WK * SEG * 4 <= (int)sizeof(smem), "LDS of the join");
+    float* sf = reinterpret_cast<float*>(smem);
+    float* mine = sf + wk * (ND * 1024);
+    float* ml = sf + WK * ND * 1024;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mine[(d * 16 + e) * 64 + lane] = acc[d][0][e];
+    if (h == 0) {
+      ml[(wk * 32 + c) * 2] = m[0];
+      ml[(wk * 32 + c) * 2 + 1] = l[0];
+    }
+    __syncthreads();
+    float mn = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WK; ++w) mn = fmaxf(mn, ml[(w * 32 + c) * 2]);
+    const float ms = mn == -INFINITY ? 0.f : mn;
+    float f[WK], ls = 0.f;
+#pragma unroll
+    for (int w = 0; w < WK; ++w) {
+      f[w] = exp2_(ml[(w * 32 + c) * 2] - ms);
+      ls += ml[(w * 32 + c) * 2 + 1] * f[w];
+    }
+    m[0] = mn;
+    l[0] = ls;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      if (d % WK != wk) continue;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        float a = 0.f;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) a += sf[(w * ND * 16 + d * 16 + e) * 64 + lane] * f[w];
+        acc[d][0][e] = a;
+      }
+    }
+  }
+
+#pragma unroll
+  for (int u = 0; u < QT; ++u) {
+    const int r = rb * BR + (wr * QT + u) * 32 + c;
+    const bool ok = r < p.M;
+    const int64_t row = (int64_t)bh * p.M + r;
+    if (p.splits > 1) {
+      const int64_t part = (int64_t)sp * bhn * p.M + row;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        if (WK > 1 && d % WK != wk) continue;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (ok) {
+            const int ch = 32 * d + 8 * q + 4 * h;
+            *reinterpret_cast<float4*>(p.ws_o + part * DP + ch) =
+                make_float4(acc[d][u][4 * q], acc[d][u][4 * q + 1], acc[d][u][4 * q + 2], acc[d][u][4 * q + 3]);
+          }
+      }
+      if (ok && h == 0 && wk == 0) {
+        p.ws_ml[part * 2] = m[u];
+        p.ws_ml[part * 2 + 1] = l[u];
+      }
+      continue;
+    }
+    const float inv = l[u] == 0.f ? 0.f : 1.f / l[u];
+    bf16_t* o = reinterpret_cast<bf16_t*>(p.o.p) + b * p.o.sb + ri[u] * p.o.ss + (hk * p.G + rg[u]) * p.o.sh;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      if (WK > 1 && d % WK != wk) continue;
+      store_row<T>(o, acc[d][u], inv, d, p.D, h, ok);
+    }
+    if (ok && h == 0 && wk == 0 && p.lse2)
+      p.lse2[row] = l[u] == 0.f ? INFINITY : m[u] + __builtin_amdgcn_logf(l[u]);
+  }
+}
+
+// joins the key splits of a row: one thread per 4 channels
+template <class T, int DP>
+__global__ __launch_bounds__(256) void attn_join_kernel(const AttnParams p) {
+  constexpr int TPR = DP / 4;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)p.B * p.Hkv * p.M;
+  const int64_t row = id / TPR;
+  const int d = (int)(id % TPR) * 4;
+  if (row >= rows) return;
+  float mn = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) mn = fmaxf(mn, p.ws_ml[(s * rows + row) * 2]);
+  const float ms = mn == -INFINITY ? 0.f : mn;
+  float l = 0.f, a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
+  for (int s = 0; s < p.splits; ++s) {
+    const float f = exp2_(p.ws_ml[(s * rows + row) * 2] - ms);
+    l += p.ws_ml[(s * rows + row) * 2 + 1] * f;
+    const float4 v = *reinterpret_cast<const float4*>(p.ws_o + (s * rows + row) * DP + d);
+    a0 += v.x * f; a1 += v.y * f; a2 += v.z * f; a3 += v.w * f;
+  }
+  const int bh = (int)(row / p.M), r = (int)(row - (int64_t)bh * p.M), b = bh / p.Hkv, hk = bh - b * p.Hkv;
+  const int i = fdiv(r, p.div_g), g = r - i * p.G;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (d < p.D) {
+    bf16_t* o = reinterpret_cast<bf16_t*>(p.o.p) + b * p.o.sb + i * p.o.ss + (hk * p.G + g) * p.o.sh + d;
+    *reinterpret_cast<uint2*>(o) = make_uint2(T::pack2(a0 * inv, a1 * inv), T::pack2(a2 * inv, a3 * inv));
+  }
+  if (d == 0 && p.lse2) p.lse2[row] = l == 0.f ? INFINITY : mn + __builtin_amdgcn_logf(l);
+}
+
+// mask bytes -> words: one wave per (32 mask rows, 64 keys)
+__global__ __launch_bounds__(256) void attn_mask_kernel(const AttnMaskArgs a) {
+  const int nib = (a.Im + 31) >> 5, lane = threadIdx.x & 63;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), per = (int64_t)nib * a.words;
+  if (unit >= per * a.Bm * a.Hm) return;
+  const int64_t lead = unit / per;
+  const int ib = (int)((unit - lead * per) / a.words), w = (int)(unit % a.words);
+  const int b = (int)(lead / a.Hm), h = (int)(lead % a.Hm), key = 64 * w + lane;
+  const uint8_t* src = a.src + b * a.sb + h * a.sh + (int64_t)imin(key, a.Sk - 1) * a.sk;
+  unsigned long long any = 0, all = ~0ull;
+  const int n = imin(32, a.Im - 32 * ib);
+#pragma unroll 8
+  for (int k = 0; k < n; ++k) {
+    const int i = 32 * ib + k;
+    const unsigned long long bits = __ballot(key < a.Sk && src[(int64_t)i * a.si] != 0);
+    any |= bits;
+    all &= bits;
+    if (lane == 0) a.bits[(lead * a.Im + i) * a.words + w] = bits;
+  }
+  if (lane == 0) a.cls[unit] = any == 0 ? 0 : all == ~0ull ? 2 : 1;
+}
+
+template <class T, int DP, int QT, int WR, int WK, int KW>
+void launch(const AttnParams& p, hipStream_t st) {
+  const int64_t n = (int64_t)((p.M + 32 * QT * WR - 1) / (32 * QT * WR)) * p.B * p.Hkv * p.splits;
+  if (p.mask.bits)
+    attn_fwd_kernel<T, DP, QT, WR, WK, KW, true><<<(unsigned)n, 64 * WR * WK, 0, st>>>(p);
+  else
+    attn_fwd_kernel<T, DP, QT, WR, WK, KW, false><<<(unsigned)n, 64 * WR * WK, 0, st>>>(p);
+}
+
+template <class T, int DP>
+void fwd(const AttnParams& p, hipStream_t st) {
+  if (p.M <= 32) {
+    launch<T, DP, 1, 1, 4, 32>(p, st);
+    if (p.splits > 1) {
+      const int64_t n = (int64_t)p.B * p.Hkv * p.M * (DP / 4);
+      attn_join_kernel<T, DP><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(p);
+    }
+  } else {
+    launch<T, DP, 1, 4, 1, 64>(p, st);
+  }
+}
+
+template <class T>
+void fwd_d(const AttnParams& p, hipStream_t st) {
+  if (p.D <= 32) fwd<T, 32>(p, st);
+  else if (p.D <= 64) fwd<T, 64>(p, st);
+  else if (p.D <= 96) fwd<T, 96>(p, st);
+  else fwd<T, 128>(p, st);
+}
+
+}  // namespace
+
+int attn_mask_bits(const AttnMaskArgs& a, hipStream_t st) {
+  const int64_t units = (int64_t)a.Bm * a.Hm * ((a.Im + 31) / 32) * a.words;
+  if (units == 0) return 0;
+  if ((units + 3) / 4 > 0x7fffffff) return 1;
+  attn_mask_kernel<<<(unsigned)((units + 3) / 4), 256, 0, st>>>(a);
+  return hipGetLastError() == hipSuccess ? 0 : 3;
+}
+
+int attn_splits(int B, int Hkv, int M, int Sk) {
+  if (M > 32) return 1;
+  const int64_t blocks = (int64_t)B * Hkv;
+  const int tiles = (Sk + 127) / 128;
+  const int64_t want = (1024 + blocks - 1) / blocks;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(want, tiles / 2));
+}
+
+int attn_fwd(const AttnParams& p, hipStream_t st) {
+  if (p.D < 8 || p.D > 128 || p.D % 8 || p.M < 1 || p.Sk < 0 || p.splits < 1) return 1;
+  const int64_t grid = ((int64_t)p.M + 31) / 32 * p.B * p.Hkv * p.splits;
+  if (grid > 0x7fffffff) return 2;
+  if (p.fp16) fwd_d<FP16>(p, st);
+  else fwd_d<BF16>(p, st);
+  return hipGetLastError() == hipSuccess ? 0 : 3;
+}

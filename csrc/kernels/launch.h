@@ -604,6 +604,105 @@ int cfl_ts_upload_pw(void* buf, int cap);
 int cfl_ts_upload_pw_bwd(void* buf, int cap);
 int cfl_ts_upload_sepconv(void* buf, int cap);
 
+// ---------------------------------------------------------------- attention (attention.hip / attention_bwd.hip)
+// x / d for 0 <= x < 2^31 as a multiplication: m = 0 -> a shift by s, else mulhi(x, m) >> s
+struct FastDiv {
+  uint32_t m, s;
+};
+inline FastDiv fast_div(uint32_t d) {
+  uint32_t s = 31 - __builtin_clz(d);
+  if ((d & (d - 1)) == 0) return FastDiv{0, s};
+  // m d - 2^(32 + s) <= d < 2^(s + 1): exact for x < 2^31
+  return FastDiv{(uint32_t)((1ull << (32 + s)) / d + 1), s};
+}
+
+__device__ __forceinline__ int fdiv32(int x, const FastDiv& f) {
+  return f.m == 0 ? x >> f.s : (int)(__umulhi((uint32_t)x, f.m) >> f.s);
+}
+
+struct AttnTensor {        // token tensor [B][S][H][D], channels contiguous; strides in elements
+  void* p;
+  int64_t sb, ss, sh;
+};
+
+// A boolean mask packed by attn_mask_bits: a word of 64 keys per (row of the mask, key tile), and a class per (32 mask
+// rows, key tile): 0 = no pair allowed, 2 = every pair allowed, 1 = some. Broadcast axes keep one entry (stride 0).
+struct AttnMask {
+  const unsigned long long* bits;   // nullptr: no mask
+  const uint8_t* cls;
+  int64_t sb, sh;                   // mask rows from one image / head to the next (0: broadcast)
+  int rows;                         // Sq, or 1: the same for every query
+  int words;                        // key tiles
+};
+
+struct AttnParams {
+  AttnTensor q, k, v, o;            // o: forward output
+  AttnTensor go, dq, dk, dv;        // backward
+  float* lse2;                      // [B][Hkv][M] log2 of the row's exp2 sum (+inf: empty row); saved for the backward
+  float* delta;                     // [B][Hkv][M] workspace of the backward
+  AttnMask mask;
+  const int* lengths;               // [B] valid keys or nullptr
+  int B, Sq, Sk, Hq, Hkv, G, D, M;  // M = Sq * G
+  int causal;
+  int fp16;
+  float scale;
+  FastDiv div_g;
+  int splits;                       // forward: key splits; partial results in ws
+  float* ws_o;                      // [splits][B][Hkv][M][DP]
+  float* ws_ml;                     // [splits][B][Hkv][M][2]
+};
+
+struct AttnMaskArgs {
+  const uint8_t* src;               // bool [Bm][Hm][Im][Sk] with strides
+  int64_t sb, sh, si, sk;
+  int Bm, Hm, Im, Sk, words;
+  unsigned long long* bits;         // [Bm][Hm][Im][words]
+  uint8_t* cls;                     // [Bm][Hm][(Im + 31) / 32][words]
+};
+
+int attn_mask_bits(const AttnMaskArgs& a, hipStream_t st);
+int attn_splits(int B, int Hkv, int M, int Sk);      // key splits of a forward call (1: no workspace)
+int attn_fwd(const AttnParams& p, hipStream_t st);
+int attn_bwd(const AttnParams& p, hipStream_t st);
+
+// ---------------------------------------------------------------- layer_norm.hip
+constexpr int LAYER_NORM_MAX_C = 16384;       // a row is held in registers: 1,024 lanes of 16
+struct LayerNormParams {
+  const void* x;           // [rows][C], row stride x_stride
+  const void* gy;          // backward
+  const float* w;          // [C] or nullptr (ones)
+  const float* b;          // [C] or nullptr (zeros); forward only
+  void* y;                 // forward: y, backward: dx (nullptr: not wanted); contiguous
+  float* dw;               // backward: [C] or nullptr
+  float* db;
+  float* ws;               // [blocks][2][C] partial dw, db
+  int64_t rows, x_stride, gy_stride;
+  int C;
+  float eps;
+  int type;                // 0 = fp32, 1 = bf16, 2 = fp16
+  int blocks;
+};
+int layer_norm_fwd(const LayerNormParams& p, hipStream_t st);
+int layer_norm_bwd_blocks(int64_t rows, int C);
+int layer_norm_bwd(const LayerNormParams& p, hipStream_t st);
+
+// ---------------------------------------------------------------- rotary.hip
+struct RotaryParams {
+  const void* x;           // [B][S][H][D] channels contiguous, strides in elements
+  void* y;                 // the same with its own strides
+  const void* pos;         // [A][B or 1][S]
+  int64_t x_sb, x_ss, x_sh, y_sb, y_ss, y_sh;
+  int64_t p_sa, p_sb, p_ss;
+  int B, S, H, D;
+  int half;                // rotated pairs
+  int end[4];              // pairs below end[a] (and at or above end[a - 1]) turn by axis a
+  double log2_theta;
+  int joint, interleaved, inverse;
+  int type;                // 0 = fp32, 1 = bf16, 2 = fp16
+  int pos_type;            // 0 = int32, 1 = int64, 2 = float32
+};
+int rotary_apply(const RotaryParams& p, hipStream_t st);
+
 // ---------------------------------------------------------------- misc (optim.hip / datagen.hip)
 int fill_f32(float* p, float v, int64_t n, hipStream_t st);
 int gather_rows_u8(const uint8_t* src, const int32_t* idx, uint8_t* dst, int rows, int64_t row_bytes,
