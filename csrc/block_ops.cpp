@@ -173,8 +173,13 @@ AttnParams params(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
   p.fp16 = q.scalar_type() == at::kHalf;
   p.scale = (float)scale;
   p.div_g = fast_div(p.G);
-  p.splits = 1;
+  p.splits = p.kv_splits = 1;
   return p;
+}
+
+// blocks of different work (attention.h locate())
+bool uneven(const AttnParams& p) {
+  return p.lengths || p.mask.sb || p.causal;
 }
 
 // The forward call on readable tensors. lse2: defined -> filled.
@@ -194,14 +199,15 @@ void run_forward(AttnParams& p, const at::Tensor& out, const at::Tensor& lse2) {
 
 // what the forward pass leaves for the backward pass, next to q, k, v and out
 struct Saved {
-  at::Tensor lse2, bits, lengths;
+  at::Tensor lse2, rest, bits, lengths;
   PackedMask pm;
 };
 
 at::Tensor forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const Shape& s, const OptT& mask,
-                   const OptT& lengths, bool causal, double scale, bool keep, Saved& sv) {
+                   const OptT& lengths, bool causal, double scale, bool lse, bool grad, Saved& sv) {
   at::Tensor out = at::empty({s.B, s.Sq, s.Hq, s.D}, q.options());
-  if (keep) sv.lse2 = at::empty({s.B, s.Hkv, s.Sq * (s.Hq / s.Hkv)}, q.options().dtype(at::kFloat));
+  if (grad) sv.rest = at::empty_like(out);
+  if (lse || grad) sv.lse2 = at::empty({s.B, s.Hkv, s.Sq * (s.Hq / s.Hkv)}, q.options().dtype(at::kFloat));
   if (out.numel() == 0) return out;
   if (lengths) sv.lengths = lengths->contiguous();
   AttnParams p = params(q, k, v, s, causal, scale, sv.lengths);
@@ -210,6 +216,8 @@ at::Tensor forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v
     sv.bits = sv.pm.buf;
     p.mask = mask_view(sv.bits, sv.pm.Bm, sv.pm.Hm, sv.pm.Im, sv.pm.words);
   }
+  p.uneven = uneven(p);
+  p.o_rest = grad ? reinterpret_cast<bf16_t*>(sv.rest.data_ptr()) : nullptr;
   run_forward(p, out, sv.lse2);
   return out;
 }
@@ -220,12 +228,23 @@ void backward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, con
   const at::Tensor go = readable(go_in);
   AttnParams p = params(q, k, v, s, causal, scale, sv.lengths);
   p.mask = mask_view(sv.bits, sv.pm.Bm, sv.pm.Hm, sv.pm.Im, sv.pm.words);
+  p.uneven = uneven(p);
   p.o = view(out);
+  p.o_rest = reinterpret_cast<bf16_t*>(sv.rest.data_ptr());
   p.go = view(go);
   if (dq.defined()) p.dq = view(dq);
   if (dk.defined()) p.dk = view(dk);
   if (dv.defined()) p.dv = view(dv);
   const at::Tensor delta = at::empty_like(sv.lse2);
+  attn_bwd_splits(p.B, p.Hkv, p.M, p.Sk, p.causal, p.splits, p.kv_splits);
+  const int64_t dp = (p.D + 31) / 32 * 32, bh = (int64_t)p.B * p.Hkv;
+  const int64_t nq = p.splits > 1 ? p.splits * bh * p.M * dp : 0, nk = p.kv_splits > 1 ? 2 * p.kv_splits * bh * p.Sk * dp : 0;
+  at::Tensor ws;
+  if (nq + nk > 0) {
+    ws = at::empty({nq + nk}, sv.lse2.options());
+    p.ws_o = ws.data_ptr<float>();
+    p.ws_kv = p.ws_o + nq;
+  }
   p.lse2 = sv.lse2.data_ptr<float>();
   p.delta = delta.data_ptr<float>();
   ok(attn_bwd(p, stream()), "attention backward");
@@ -261,8 +280,8 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
     const Shape s{q.size(0), q.size(1), k.size(1), q.size(2), k.size(2), q.size(3)};
     const at::Tensor qr = readable(q), kr = readable(k), vr = readable(v);
     Saved sv;
-    const at::Tensor out = ::forward(qr, kr, vr, s, mask, lengths, causal, scale, true, sv);
-    ctx->save_for_backward({qr, kr, vr, out, sv.lse2, sv.bits, sv.lengths});
+    const at::Tensor out = ::forward(qr, kr, vr, s, mask, lengths, causal, scale, true, true, sv);
+    ctx->save_for_backward({qr, kr, vr, out, sv.lse2, sv.rest, sv.bits, sv.lengths});
     put_meta(ctx, s, causal, scale, sv.pm);
     ctx->mark_non_differentiable({sv.lse2});
     return {out, sv.lse2};
@@ -276,8 +295,9 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
     Saved sv;
     get_meta(ctx, s, causal, scale, sv.pm);
     sv.lse2 = t[4];
-    sv.bits = t[5];
-    sv.lengths = t[6];
+    sv.rest = t[5];
+    sv.bits = t[6];
+    sv.lengths = t[7];
     variable_list r(7);
     const c10::DeviceGuard guard(t[0].device());
     for (int i = 0; i < 3; ++i)
@@ -300,8 +320,8 @@ struct AttentionQkvFn : torch::autograd::Function<AttentionQkvFn> {
     const Shape s{t.size(0), t.size(1), t.size(1), heads, kv, t.size(3)};
     Saved sv;
     const at::Tensor out = ::forward(t.narrow(2, 0, heads), t.narrow(2, heads, kv), t.narrow(2, heads + kv, kv), s,
-                                     mask, lengths, causal, scale, true, sv);
-    ctx->save_for_backward({t, out, sv.lse2, sv.bits, sv.lengths});
+                                     mask, lengths, causal, scale, true, true, sv);
+    ctx->save_for_backward({t, out, sv.lse2, sv.rest, sv.bits, sv.lengths});
     put_meta(ctx, s, causal, scale, sv.pm);
     ctx->mark_non_differentiable({sv.lse2});
     return {out, sv.lse2};
@@ -315,8 +335,9 @@ struct AttentionQkvFn : torch::autograd::Function<AttentionQkvFn> {
     Saved sv;
     get_meta(ctx, s, causal, scale, sv.pm);
     sv.lse2 = t[2];
-    sv.bits = t[3];
-    sv.lengths = t[4];
+    sv.rest = t[3];
+    sv.bits = t[4];
+    sv.lengths = t[5];
     const c10::DeviceGuard guard(t[0].device());
     const at::Tensor d = at::empty(t[0].sizes(), t[0].options());
     if (d.numel() != 0) {
@@ -348,7 +369,7 @@ py::object attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor&
   }
   Saved sv;
   const at::Tensor out =
-      forward(readable(q), readable(k), readable(v), s, mask, lengths, causal, sc, return_lse, sv);
+      forward(readable(q), readable(k), readable(v), s, mask, lengths, causal, sc, return_lse, false, sv);
   return result(out, sv.lse2, s, return_lse);
 }
 
@@ -368,7 +389,7 @@ py::object attention_qkv(const at::Tensor& qkv, int64_t heads, std::optional<int
   }
   Saved sv;
   const at::Tensor out =
-      forward(readable(q), readable(k), readable(v), s, mask, lengths, causal, sc, return_lse, sv);
+      forward(readable(q), readable(k), readable(v), s, mask, lengths, causal, sc, return_lse, false, sv);
   return result(out, sv.lse2, s, return_lse);
 }
 

@@ -14,6 +14,8 @@
 #include "common.h"
 #include "launch.h"
 
+#include <type_traits>
+
 namespace attn {
 
 constexpr float LOG2E = 1.4426950408889634f;
@@ -24,6 +26,7 @@ typedef _Float16 h8v __attribute__((ext_vector_type(8)));
 typedef _Float16 h2v __attribute__((ext_vector_type(2)));
 
 struct BF16 {
+  static constexpr short INF = 0x7f80, ONE = 0x3f80;
   static CFL_DEVICE f16v mma(const s8v& a, const s8v& b, const f16v& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8v, a), __builtin_bit_cast(bf8v, b), c, 0, 0,
                                                    0);
@@ -34,6 +37,7 @@ struct BF16 {
 };
 
 struct FP16 {
+  static constexpr short INF = 0x7c00, ONE = 0x3c00;
   static CFL_DEVICE f16v mma(const s8v& a, const s8v& b, const f16v& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
   }
@@ -44,6 +48,9 @@ struct FP16 {
   static CFL_DEVICE float lo(uint32_t w) { return (float)__builtin_bit_cast(h2v, w)[0]; }
   static CFL_DEVICE float hi(uint32_t w) { return (float)__builtin_bit_cast(h2v, w)[1]; }
 };
+
+// what a call allows: every key up to the image's length; the causal ones of those; a boolean mask, causal or not
+enum Kind { ATTN_PLAIN = 0, ATTN_CAUSAL = 1, ATTN_MASK = 2 };
 
 CFL_DEVICE int rowof(int e, int h) { return (e & 3) + 8 * (e >> 2) + 4 * h; }
 
@@ -68,10 +75,12 @@ CFL_DEVICE int swz(int row) {
 template <int DP>
 CFL_DEVICE int lds_at(int row, int chunk) { return row * DP + ((chunk ^ swz<DP>(row)) << 3); }
 
-// A operand of a product that reduces over d: row `row`, chunk = 2 * kk + h
+// A operand of a product that reduces over d: fragment kk of the token row whose chunk h is at element `at` of the tile
+// (lds_at of row c; rows 32 apart are permuted alike)
 template <int DP>
-CFL_DEVICE s8v frag(const bf16_t* tile, int row, int chunk) {
-  return *reinterpret_cast<const s8v*>(tile + lds_at<DP>(row, chunk));
+CFL_DEVICE s8v frag_x(const bf16_t* tile, int at, int kk) {
+  if (DP % 64 == 0) return *reinterpret_cast<const s8v*>(tile + (at ^ (kk << 4)));
+  return *reinterpret_cast<const s8v*>(tile + (at ^ ((kk & 1) << 4)) + ((kk >> 1) << 5));
 }
 
 CFL_DEVICE s4v tr4(const bf16_t* p) {
@@ -89,6 +98,47 @@ CFL_DEVICE s8v frag_t(const bf16_t* tile, int row0, int dt, int lane) {
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+// Values that are not finite, where pairs are not allowed. A product over token rows gives such a pair the factor 0, but
+// 0 * inf and 0 * NaN are NaN: what a key holds where no query may attend it would show in every row. So after its walk
+// a block with any mask looks whether its sums are finite (they are, in all but broken calls) and if not walks again
+// with the operand's values replaced by 0 (clean), and those of pairs with a probability put back: `poison` adds +inf /
+// -inf to the sums whose pairs of p > 0 hold +inf or NaN / -inf or NaN (both: NaN).
+template <class T>
+CFL_DEVICE s8v clean(const s8v& a, s8v& pos, s8v& neg) {
+  s8v r;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const short m = (short)(a[j] & 0x7fff);
+    const bool fin = m < T::INF, nan = m > T::INF;
+    r[j] = fin ? a[j] : (short)0;
+    pos[j] = !fin && (nan || a[j] >= 0) ? T::ONE : (short)0;
+    neg[j] = !fin && (nan || a[j] < 0) ? T::ONE : (short)0;
+  }
+  return r;
+}
+template <class T>
+CFL_DEVICE void poison(f16v& acc, const s8v& pos, const s8v& neg, const s8v& p) {
+  s8v one;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) one[j] = p[j] != 0 ? T::ONE : (short)0;
+  f16v z;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) z[e] = 0.f;
+  const f16v a = T::mma(pos, one, z);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] += a[e] > 0.f ? INFINITY : 0.f;
+  const f16v b = T::mma(neg, one, z);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] -= b[e] > 0.f ? INFINITY : 0.f;
+}
+// 0, or NaN if any element is not finite
+CFL_DEVICE float finite_sum(const f16v& v) {
+  float t = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) t = fmaf(v[e], 0.f, t);
+  return t;
+}
+
 // eight elements 8s .. 8s + 7 of a result, rounded to 16 bits: the B operand of the second product
 template <class T>
 CFL_DEVICE s8v pack_b(const f16v& v, int s) {
@@ -98,20 +148,40 @@ CFL_DEVICE s8v pack_b(const f16v& v, int s) {
 }
 
 // 32 channels 32 * dt .. + 31 of one token row per lane pair (c, c + 32): four quads each, exchanged between the
-// halves so that a lane stores 16 contiguous bytes (lane half h: channels 16s + 8h .. + 7)
+// halves so that a lane stores 16 contiguous bytes (lane half h: channels 16s + 8h .. + 7). rest: if given, what the
+// rounding took away, rounded itself.
 template <class T>
-CFL_DEVICE void store_row(bf16_t* row, const f16v& v, float mul, int dt, int D, int h, bool ok) {
+CFL_DEVICE void store_row(bf16_t* row, const f16v& v, float mul, int dt, int D, int h, bool ok,
+                          bf16_t* rest = nullptr) {
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
-    const unsigned a0 = T::pack2(v[8 * s] * mul, v[8 * s + 1] * mul);
-    const unsigned a1 = T::pack2(v[8 * s + 2] * mul, v[8 * s + 3] * mul);
-    const unsigned b0 = T::pack2(v[8 * s + 4] * mul, v[8 * s + 5] * mul);
-    const unsigned b1 = T::pack2(v[8 * s + 6] * mul, v[8 * s + 7] * mul);
-    const auto x = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
-    const auto y = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
+    unsigned w[4], x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float a = v[8 * s + 2 * j] * mul, b = v[8 * s + 2 * j + 1] * mul;
+      w[j] = T::pack2(a, b);
+      x[j] = T::pack2(a - T::lo(w[j]), b - T::hi(w[j]));
+    }
     const int d = 32 * dt + 16 * s + 8 * h;
-    if (ok && d < D) *reinterpret_cast<uint4*>(row + d) = make_uint4(x[0], y[0], x[1], y[1]);
+    const auto p = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+    const auto q = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+    if (ok && d < D) *reinterpret_cast<uint4*>(row + d) = make_uint4(p[0], q[0], p[1], q[1]);
+    if (rest != nullptr) {
+      const auto y = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false);
+      const auto z = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
+      if (ok && d < D) *reinterpret_cast<uint4*>(rest + d) = make_uint4(y[0], z[0], y[1], z[1]);
+    }
   }
+}
+
+// the same channels of a part of a sum, fp32, rows of DP
+template <int DP>
+CFL_DEVICE void store_part(float* row, const f16v& v, float mul, int dt, int h, bool ok) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    if (ok)
+      *reinterpret_cast<float4*>(row + 32 * dt + 8 * q + 4 * h) =
+          make_float4(v[4 * q] * mul, v[4 * q + 1] * mul, v[4 * q + 2] * mul, v[4 * q + 3] * mul);
 }
 
 // 16 bytes of the buffer at byte offset `off` -> LDS at the wave-uniform `lds` + 16 * lane; an offset past the range
@@ -146,55 +216,74 @@ CFL_DEVICE u4v rsrc(const void* base) {
 
 CFL_DEVICE int fdiv(int x, const FastDiv& f) { return fdiv32(x, f); }
 
-// Which tiles of a walk hold any allowed pair, and which only allowed ones, for the block: lanes look up the classes of
-// 64 tiles ahead at a time, two ballots keep them.
-struct TileMask {
-  unsigned long long live, whole;
-  int base;
-  int64_t lead0, leadg;          // class rows of this block's first head, and from one head to the next
-  int heads, nib;
-
-  CFL_DEVICE void init(const AttnParams& p, int b, int hk) {
-    nib = (p.mask.rows + 31) >> 5;
-    // sb / sh count mask rows, `rows` of them for each (image, head) entry
-    lead0 = (b * p.mask.sb + (int64_t)hk * p.G * p.mask.sh) / p.mask.rows;
-    leadg = p.mask.sh ? 1 : 0;
-    heads = p.mask.sh ? p.G : 1;
-    base = -64;
-    live = whole = 0;
+// Which of `n` blocks of an (image, key head), which of bhn of those and which of `splits` parts this workgroup is.
+// Where all blocks have the same work, XCD by XCD: the blocks that read one head's tokens share an L2 (16 heads, 4,096
+// tokens, 128 channels: 292 us forward against 302). Where they differ (causal: block 0 must be the longest; lengths;
+// masks by image) that order gives some XCDs the long ones: then block by block over all heads, the longest first, the
+// heads rotated so that no XCD keeps one (the same shape, causal: 157 us against 199).
+CFL_DEVICE void locate(const AttnParams& p, int n, int bhn, int splits, int& blk, int& bh, int& sp) {
+  const int heads = bhn * splits;
+  int rest;
+  if (p.uneven) {
+    blk = (int)blockIdx.x / heads;
+    rest = ((int)blockIdx.x - blk * heads + blk) % heads;
+  } else {
+    const int lin = xcd_swizzle(blockIdx.x, gridDim.x);
+    rest = lin / n;
+    blk = lin - rest * n;
   }
-  // 0 / 1 / 2 as the mask's classes, over queries i0 .. i1 and words w0 .. w1 (this lane's tile; `in`: it exists)
-  CFL_DEVICE int cls(const AttnParams& p, int i0, int i1, int w0, int w1, bool in) const {
-    bool any = false, all = true;
-    if (in) {
-      const int b0 = p.mask.rows > 1 ? i0 >> 5 : 0, b1 = p.mask.rows > 1 ? i1 >> 5 : 0;
-      for (int g = 0; g < heads; ++g)
-        for (int ib = b0; ib <= b1; ++ib)
-          for (int w = w0; w <= w1; ++w) {
-            const int k = p.mask.cls[((lead0 + g * leadg) * nib + ib) * p.mask.words + w];
-            any |= k != 0;
-            all &= k == 2;
-          }
+  sp = rest / bhn;
+  bh = rest - sp * bhn;
+}
+
+// Which tiles of a block's walk hold any allowed pair, and which only allowed ones: a byte a tile in LDS, filled from the
+// mask's classes at the start. Tiles past the table count as partly allowed.
+constexpr int MASK_TILES = 2048;
+struct TileMask {
+  const uint8_t* tab;            // MASK_TILES + 64 bytes
+  bool part;                     // the tile that next() returned holds pairs that are not allowed
+
+  // f(t, i0, i1, w0, w1): queries i0 .. i1 and mask words w0 .. w1 of tile t
+  template <class F>
+  CFL_DEVICE void fill(const AttnParams& p, int b, int hk, uint8_t* t8, int tiles, const F& f) {
+    tab = t8;
+    const int nib = (p.mask.rows + 31) >> 5, heads = p.mask.sh ? p.G : 1;
+    // sb / sh count mask rows, `rows` of them for each (image, head) entry
+    const int64_t lead = (b * p.mask.sb + (int64_t)hk * p.G * p.mask.sh) / p.mask.rows;
+    for (int t = threadIdx.x; t < MASK_TILES + 64; t += blockDim.x) {
+      bool any = false, all = true;
+      if (t < tiles && t < MASK_TILES) {
+        int i0, i1, w0, w1;
+        f(t, i0, i1, w0, w1);
+        const int b0 = p.mask.rows > 1 ? i0 >> 5 : 0, b1 = p.mask.rows > 1 ? i1 >> 5 : 0;
+        for (int g = 0; g < heads; ++g)
+          for (int ib = b0; ib <= b1; ++ib)
+            for (int w = w0; w <= w1; ++w) {
+              const int k = p.mask.cls[((lead + g) * nib + ib) * p.mask.words + w];
+              any |= k != 0;
+              all &= k == 2;
+            }
+      }
+      t8[t] = any ? (all ? 2 : 1) : 0;
     }
-    return any ? (all ? 2 : 1) : 0;
+    __syncthreads();
   }
   // first tile at or after t with an allowed pair, t1 if there is none before it
-  template <class F>
-  CFL_DEVICE int next(int t, int t1, const F& f) {
+  CFL_DEVICE int next(int t, int t1) {
+    part = true;
     while (t < t1) {
-      if (t - base >= 64) {
-        const int k = f(t + (int)(threadIdx.x & 63));
-        live = __ballot(k != 0);
-        whole = __ballot(k == 2);
-        base = t;
+      if (t >= MASK_TILES) return t;
+      const int k = tab[t + (int)(threadIdx.x & 63)];
+      const unsigned long long live = __ballot(k != 0), whole = __ballot(k == 2);
+      if (live) {
+        const int n = __builtin_ctzll(live);
+        part = !((whole >> n) & 1);
+        return imin(t + n, t1);
       }
-      const unsigned long long rest = live >> (t - base);
-      if (rest) return imin(t + __builtin_ctzll(rest), t1);
-      t = base + 64;
+      t = imin(t + 64, imax(t + 1, MASK_TILES));
     }
     return t1;
   }
-  CFL_DEVICE bool is_whole(int t) const { return (whole >> ((t - base) & 63)) & 1; }
 };
 
 }  // namespace attn

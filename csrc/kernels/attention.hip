@@ -20,11 +20,16 @@ using namespace attn;
 // precision is the same) and most tiles rescale nothing
 constexpr float SLACK = 8.f;
 
+// up to this many rows the four waves of a block split the keys of a tile, beyond it the rows
+constexpr int FEW_ROWS = 32;
+
 // QT: 32-row tiles per wave; WR x WK: waves along the rows and along the keys of a tile; KW keys per wave and tile
-template <class T, int DP, int QT, int WR, int WK, int KW, bool MASK>
-__global__ __launch_bounds__(64 * WR * WK) void attn_fwd_kernel(const AttnParams p) {
+template <class T, int DP, int QT, int WR, int WK, int KW, int MINW, int KIND>
+__global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const AttnParams p) {
   constexpr int NT = 64 * WR * WK, KT = KW * WK, TILE = KT * DP, CPR = DP / 8, CH = KT * CPR / NT;
   constexpr int NK = KW / 32, NKK = DP / 16, ND = DP / 32;
+  constexpr bool MASK = KIND == ATTN_MASK;
+  const bool causal = KIND == ATTN_CAUSAL || (MASK && p.causal);
   static_assert(KT * CPR % NT == 0, "whole DMA instructions");
   __shared__ __attribute__((aligned(1024))) bf16_t smem[4 * TILE];
 
@@ -32,12 +37,12 @@ __global__ __launch_bounds__(64 * WR * WK) void attn_fwd_kernel(const AttnParams
   const int c = lane & 31, h = lane >> 5, wr = wid / WK, wk = wid % WK;
   constexpr int BR = 32 * QT * WR;
   const int nrb = (p.M + BR - 1) / BR, bhn = p.B * p.Hkv;
-  const int lin = xcd_swizzle(blockIdx.x, gridDim.x);
-  const int rb0 = lin % nrb, rest = lin / nrb, bh = rest % bhn, sp = rest / bhn;
-  const int rb = p.causal ? nrb - 1 - rb0 : rb0;          // causal: long rows first
+  int rb0, bh, sp;
+  locate(p, nrb, bhn, p.splits, rb0, bh, sp);
+  const int rb = causal ? nrb - 1 - rb0 : rb0;          // causal: long rows first
   const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const int len = p.lengths ? imin(imax(p.lengths[b], 0), p.Sk) : p.Sk;
-  const int off = p.causal ? p.Sk - p.Sq : 0;
+  const int off = causal ? p.Sk - p.Sq : 0;
   const int r_end = imin(rb * BR + BR, p.M);
 
   // this lane's rows: their queries as B operands, and the first key each may not attend
@@ -50,7 +55,7 @@ __global__ __launch_bounds__(64 * WR * WK) void attn_fwd_kernel(const AttnParams
     const int rr = ok ? r : p.M - 1, i = fdiv(rr, p.div_g), g = rr - i * p.G;
     ri[t] = i;
     rg[t] = g;
-    lim[t] = !ok ? 0 : p.causal ? imin(imax(i + off + 1, 0), len) : len;
+    lim[t] = !ok ? 0 : causal ? imin(imax(i + off + 1, 0), len) : len;
     const bf16_t* q = reinterpret_cast<const bf16_t*>(p.q.p) + b * p.q.sb + i * p.q.ss + (hk * p.G + g) * p.q.sh;
 #pragma unroll
     for (int kk = 0; kk < NKK; ++kk) {
@@ -62,11 +67,11 @@ __global__ __launch_bounds__(64 * WR * WK) void attn_fwd_kernel(const AttnParams
   }
   // first key past every row of the block / of this wave (rows are in query order)
   const int i_last = fdiv(r_end - 1, p.div_g);
-  const int kend = p.causal ? imin(imax(i_last + off + 1, 0), len) : len;
+  const int kend = causal ? imin(imax(i_last + off + 1, 0), len) : len;
   const int wr0 = rb * BR + wr * QT * 32;
   const int wi0 = fdiv(imin(wr0, p.M - 1), p.div_g), wi1 = fdiv(imin(wr0 + QT * 32, p.M) - 1, p.div_g);
-  const int wlast = wr0 >= p.M ? 0 : p.causal ? imin(imax(wi1 + off + 1, 0), len) : len;
-  const int wfull = p.causal ? imin(imax(wi0 + off + 1, 0), len) : len;   // keys below it: allowed for every row
+  const int wlast = wr0 >= p.M ? 0 : causal ? imin(imax(wi1 + off + 1, 0), len) : len;
+  const int wfull = causal ? imin(imax(wi0 + off + 1, 0), len) : len;   // keys below it: allowed for every row
 
   const int tiles = (p.Sk + KT - 1) / KT, tps = (tiles + p.splits - 1) / p.splits;
   const int t0 = sp * tps, t1 = imin(imin(t0 + tps, tiles), (kend + KT - 1) / KT);
@@ -103,15 +108,16 @@ __global__ __launch_bounds__(64 * WR * WK) void attn_fwd_kernel(const AttnParams
       mrow[t] = p.mask.bits + (b * p.mask.sb + (hk * p.G + rg[t]) * p.mask.sh + (p.mask.rows > 1 ? ri[t] : 0)) *
                                   (int64_t)p.mask.words;
   }
+  __shared__ uint8_t classes[MASK ? MASK_TILES + 64 : 1];
   TileMask tm;
-  if (MASK) tm.init(p, b, hk);
-  const int i_first = fdiv(rb * BR, p.div_g);
-  auto next = [&](int t) {
-    if (!MASK) return t;
-    return tm.next(t, t1, [&](int u) {
-      return tm.cls(p, i_first, i_last, u * KT / 64, imin((u * KT + KT - 1) / 64, p.mask.words - 1), u < tiles);
+  if (MASK)
+    tm.fill(p, b, hk, classes, tiles, [&](int t, int& i0, int& i1, int& w0, int& w1) {
+      i0 = fdiv(rb * BR, p.div_g);
+      i1 = i_last;
+      w0 = t * KT / 64;
+      w1 = imin((t * KT + KT - 1) / 64, p.mask.words - 1);
     });
-  };
+  auto next = [&](int t) { return MASK ? tm.next(t, t1) : t; };
   auto words = [&](int t) {
     const int w = imin((t * KT + wk * KW) >> 6, p.mask.words - 1);
 #pragma unroll
@@ -120,122 +126,143 @@ __global__ __launch_bounds__(64 * WR * WK) void attn_fwd_kernel(const AttnParams
 
   f16v acc[ND][QT];
   float m[QT], l[QT];
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    m[t] = -INFINITY;
-    l[t] = 0.f;
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[d][t][e] = 0.f;
-  }
   const float sc = p.scale * LOG2E;
-
-  int t = next(t0), buf = 0;
-  if (t < t1) {
-    if (MASK) words(t);
-    issue(t, 0);
-  }
-  wait_vm();
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-  while (t < t1) {
-    const bool part = MASK && !tm.is_whole(t);
-    const int tn = next(t + 1);
-    unsigned long long cur[QT];
-    const int key0 = t * KT + wk * KW;
-    if (MASK) {
+  const int fo = lds_at<DP>(c, h);
+  auto walk = [&](auto safe) {
+    constexpr bool SAFE = decltype(safe)::value;
 #pragma unroll
-      for (int u = 0; u < QT; ++u) cur[u] = word[u] >> (key0 & 32);
-      if (tn < t1) words(tn);
+    for (int t = 0; t < QT; ++t) {
+      m[t] = -INFINITY;
+      l[t] = 0.f;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[d][t][e] = 0.f;
     }
-    if (tn < t1) issue(tn, buf ^ 1);
 
-    if (key0 < wlast) {
-      const bf16_t* sk = smem + buf * 2 * TILE + wk * KW * DP;
-      const bf16_t* sv = sk + TILE;
-      f16v s[NK][QT];
+    int t = next(t0), buf = 0;
+    if (t < t1) {
+      if (MASK) words(t);
+      issue(t, 0);
+    }
+    wait_vm();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    while (t < t1) {
+      const bool part = MASK && tm.part;
+      const int tn = next(t + 1);
+      unsigned long long cur[QT];
+      const int key0 = t * KT + wk * KW;
+      if (MASK) {
 #pragma unroll
-      for (int k = 0; k < NK; ++k)
-#pragma unroll
-        for (int u = 0; u < QT; ++u)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) s[k][u][e] = 0.f;
-#pragma unroll
-      for (int kk = 0; kk < NKK; ++kk)
-#pragma unroll
-        for (int k = 0; k < NK; ++k) {
-          const s8v a = frag<DP>(sk, 32 * k + c, 2 * kk + h);
-#pragma unroll
-          for (int u = 0; u < QT; ++u) s[k][u] = T::mma(a, qf[u][kk], s[k][u]);
-        }
-      if (MASK && part) {
-#pragma unroll
-        for (int u = 0; u < QT; ++u)
-#pragma unroll
-          for (int k = 0; k < NK; ++k) {
-            const uint32_t w = (uint32_t)(cur[u] >> (32 * k)) >> (4 * h);
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              s[k][u][e] = (w >> ((e & 3) + 8 * (e >> 2))) & 1 ? s[k][u][e] : -INFINITY;
-          }
+        for (int u = 0; u < QT; ++u) cur[u] = word[u] >> (key0 & 32);
+        if (tn < t1) words(tn);
       }
-      if (key0 + KW > wfull) {
-#pragma unroll
-        for (int u = 0; u < QT; ++u)
-#pragma unroll
-          for (int k = 0; k < NK; ++k) {
-            const int left = lim[u] - key0 - 32 * k - 4 * h;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[k][u][e] = (e & 3) + 8 * (e >> 2) < left ? s[k][u][e] : -INFINITY;
-          }
-      }
-      s8v pb[QT][2 * NK];
-#pragma unroll
-      for (int u = 0; u < QT; ++u) {
-        float mx = s[0][u][0];
+      if (tn < t1) issue(tn, buf ^ 1);
+
+      if (key0 < wlast) {
+        const bf16_t* sk = smem + buf * 2 * TILE + wk * KW * DP;
+        const bf16_t* sv = sk + TILE;
+        f16v s[NK][QT];
 #pragma unroll
         for (int k = 0; k < NK; ++k)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[k][u][e]);
-        mx = fmaxf(mx, other_half(mx)) * sc;
-        if (__any(mx > m[u] + SLACK)) {
-          const float mn = fmaxf(m[u], mx), al = exp2_(m[u] - (mn == -INFINITY ? 0.f : mn));
-          m[u] = mn;
-          l[u] *= al;
+          for (int u = 0; u < QT; ++u)
 #pragma unroll
-          for (int d = 0; d < ND; ++d)
+            for (int e = 0; e < 16; ++e) s[k][u][e] = 0.f;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[d][u][e] *= al;
-        }
-        const float ms = m[u] == -INFINITY ? 0.f : m[u];
-        float sum = 0.f;
+        for (int kk = 0; kk < NKK; ++kk)
 #pragma unroll
-        for (int k = 0; k < NK; ++k) {
+          for (int k = 0; k < NK; ++k) {
+            const s8v a = frag_x<DP>(sk + 32 * k * DP, fo, kk);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            s[k][u][e] = exp2_(fmaf(s[k][u][e], sc, -ms));
-            sum += s[k][u][e];
+            for (int u = 0; u < QT; ++u) s[k][u] = T::mma(a, qf[u][kk], s[k][u]);
           }
-          pb[u][2 * k] = pack_b<T>(s[k][u], 0);
-          pb[u][2 * k + 1] = pack_b<T>(s[k][u], 1);
+        if (MASK && part) {
+#pragma unroll
+          for (int u = 0; u < QT; ++u)
+#pragma unroll
+            for (int k = 0; k < NK; ++k) {
+              const uint32_t w = (uint32_t)(cur[u] >> (32 * k)) >> (4 * h);
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                s[k][u][e] = (w >> ((e & 3) + 8 * (e >> 2))) & 1 ? s[k][u][e] : -INFINITY;
+            }
         }
-        l[u] += sum;
+        if (key0 + KW > wfull) {
+#pragma unroll
+          for (int u = 0; u < QT; ++u)
+#pragma unroll
+            for (int k = 0; k < NK; ++k) {
+              const int left = lim[u] - key0 - 32 * k - 4 * h;
+#pragma unroll
+              for (int e = 0; e < 16; ++e) s[k][u][e] = (e & 3) + 8 * (e >> 2) < left ? s[k][u][e] : -INFINITY;
+            }
+        }
+        s8v pb[QT][2 * NK];
+#pragma unroll
+        for (int u = 0; u < QT; ++u) {
+          float mx = s[0][u][0];
+#pragma unroll
+          for (int k = 0; k < NK; ++k)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[k][u][e]);
+          mx = fmaxf(mx, other_half(mx)) * sc;
+          if (__any(mx > m[u] + SLACK)) {
+            const float mn = fmaxf(m[u], mx), al = exp2_(m[u] - (mn == -INFINITY ? 0.f : mn));
+            m[u] = mn;
+            l[u] *= al;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) acc[d][u][e] *= al;
+          }
+          const float ms = m[u] == -INFINITY ? 0.f : m[u];
+          float sum = 0.f;
+#pragma unroll
+          for (int k = 0; k < NK; ++k) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              s[k][u][e] = exp2_(fmaf(s[k][u][e], sc, -ms));
+              sum += s[k][u][e];
+            }
+            pb[u][2 * k] = pack_b<T>(s[k][u], 0);
+            pb[u][2 * k + 1] = pack_b<T>(s[k][u], 1);
+          }
+          l[u] += sum;
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2 * NK; ++ks)
+#pragma unroll
+          for (int d = 0; d < ND; ++d) {
+            s8v a = frag_t<DP>(sv, 16 * ks, d, lane);
+            if constexpr (SAFE) {
+              s8v pos, neg;
+              __builtin_amdgcn_sched_barrier(0);           // few registers matter here, not speed
+              a = clean<T>(a, pos, neg);
+#pragma unroll
+              for (int u = 0; u < QT; ++u) poison<T>(acc[d][u], pos, neg, pb[u][ks]);
+            }
+#pragma unroll
+            for (int u = 0; u < QT; ++u) acc[d][u] = T::mma(a, pb[u][ks], acc[d][u]);
+          }
       }
-#pragma unroll
-      for (int ks = 0; ks < 2 * NK; ++ks)
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          const s8v a = frag_t<DP>(sv, 16 * ks, d, lane);
-#pragma unroll
-          for (int u = 0; u < QT; ++u) acc[d][u] = T::mma(a, pb[u][ks], acc[d][u]);
-        }
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      buf ^= 1;
+      t = tn;
     }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    buf ^= 1;
-    t = tn;
+
+  };
+  walk(std::false_type{});
+  if constexpr (KIND != ATTN_PLAIN) {
+    float z = 0.f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int u = 0; u < QT; ++u) z += finite_sum(acc[d][u]);
+    if (__syncthreads_or(z != 0.f)) walk(std::true_type{});
   }
 
 #pragma unroll
@@ -294,13 +321,7 @@ __global__ __launch_bounds__(64 * WR * WK) void attn_fwd_kernel(const AttnParams
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
         if (WK > 1 && d % WK != wk) continue;
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (ok) {
-            const int ch = 32 * d + 8 * q + 4 * h;
-            *reinterpret_cast<float4*>(p.ws_o + part * DP + ch) =
-                make_float4(acc[d][u][4 * q], acc[d][u][4 * q + 1], acc[d][u][4 * q + 2], acc[d][u][4 * q + 3]);
-          }
+        store_part<DP>(p.ws_o + part * DP, acc[d][u], 1.f, d, h, ok);
       }
       if (ok && h == 0 && wk == 0) {
         p.ws_ml[part * 2] = m[u];
@@ -309,11 +330,12 @@ __global__ __launch_bounds__(64 * WR * WK) void attn_fwd_kernel(const AttnParams
       continue;
     }
     const float inv = l[u] == 0.f ? 0.f : 1.f / l[u];
-    bf16_t* o = reinterpret_cast<bf16_t*>(p.o.p) + b * p.o.sb + ri[u] * p.o.ss + (hk * p.G + rg[u]) * p.o.sh;
+    const int64_t at = b * p.o.sb + ri[u] * p.o.ss + (hk * p.G + rg[u]) * p.o.sh;
+    bf16_t *o = reinterpret_cast<bf16_t*>(p.o.p) + at, *rest = p.o_rest ? p.o_rest + at : nullptr;
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
       if (WK > 1 && d % WK != wk) continue;
-      store_row<T>(o, acc[d][u], inv, d, p.D, h, ok);
+      store_row<T>(o, acc[d][u], inv, d, p.D, h, ok, rest);
     }
     if (ok && h == 0 && wk == 0 && p.lse2)
       p.lse2[row] = l[u] == 0.f ? INFINITY : m[u] + __builtin_amdgcn_logf(l[u]);
@@ -342,8 +364,13 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnParams p) {
   const int i = fdiv(r, p.div_g), g = r - i * p.G;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   if (d < p.D) {
-    bf16_t* o = reinterpret_cast<bf16_t*>(p.o.p) + b * p.o.sb + i * p.o.ss + (hk * p.G + g) * p.o.sh + d;
-    *reinterpret_cast<uint2*>(o) = make_uint2(T::pack2(a0 * inv, a1 * inv), T::pack2(a2 * inv, a3 * inv));
+    const int64_t at = b * p.o.sb + i * p.o.ss + (hk * p.G + g) * p.o.sh + d;
+    a0 *= inv; a1 *= inv; a2 *= inv; a3 *= inv;
+    const uint2 w = make_uint2(T::pack2(a0, a1), T::pack2(a2, a3));
+    *reinterpret_cast<uint2*>(reinterpret_cast<bf16_t*>(p.o.p) + at) = w;
+    if (p.o_rest)
+      *reinterpret_cast<uint2*>(p.o_rest + at) = make_uint2(T::pack2(a0 - T::lo(w.x), a1 - T::hi(w.x)),
+                                                            T::pack2(a2 - T::lo(w.y), a3 - T::hi(w.y)));
   }
   if (d == 0 && p.lse2) p.lse2[row] = l == 0.f ? INFINITY : mn + __builtin_amdgcn_logf(l);
 }
@@ -370,25 +397,24 @@ __global__ __launch_bounds__(256) void attn_mask_kernel(const AttnMaskArgs a) {
   if (lane == 0) a.cls[unit] = any == 0 ? 0 : all == ~0ull ? 2 : 1;
 }
 
-template <class T, int DP, int QT, int WR, int WK, int KW>
+template <class T, int DP, int QT, int WR, int WK, int KW, int MINW>
 void launch(const AttnParams& p, hipStream_t st) {
   const int64_t n = (int64_t)((p.M + 32 * QT * WR - 1) / (32 * QT * WR)) * p.B * p.Hkv * p.splits;
   if (p.mask.bits)
-    attn_fwd_kernel<T, DP, QT, WR, WK, KW, true><<<(unsigned)n, 64 * WR * WK, 0, st>>>(p);
+    attn_fwd_kernel<T, DP, QT, WR, WK, KW, MINW, ATTN_MASK><<<(unsigned)n, 64 * WR * WK, 0, st>>>(p);
+  else if (p.causal)
+    attn_fwd_kernel<T, DP, QT, WR, WK, KW, MINW, ATTN_CAUSAL><<<(unsigned)n, 64 * WR * WK, 0, st>>>(p);
   else
-    attn_fwd_kernel<T, DP, QT, WR, WK, KW, false><<<(unsigned)n, 64 * WR * WK, 0, st>>>(p);
+    attn_fwd_kernel<T, DP, QT, WR, WK, KW, MINW, ATTN_PLAIN><<<(unsigned)n, 64 * WR * WK, 0, st>>>(p);
 }
 
 template <class T, int DP>
 void fwd(const AttnParams& p, hipStream_t st) {
-  if (p.M <= 32) {
-    launch<T, DP, 1, 1, 4, 32>(p, st);
-    if (p.splits > 1) {
-      const int64_t n = (int64_t)p.B * p.Hkv * p.M * (DP / 4);
-      attn_join_kernel<T, DP><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(p);
-    }
-  } else {
-    launch<T, DP, 1, 4, 1, 64>(p, st);
+  if (p.M <= FEW_ROWS) launch<T, DP, 1, 1, 4, 32, 1>(p, st);
+  else launch<T, DP, 1, 4, 1, 64, 2>(p, st);
+  if (p.splits > 1) {
+    const int64_t n = (int64_t)p.B * p.Hkv * p.M * (DP / 4);
+    attn_join_kernel<T, DP><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(p);
   }
 }
 
@@ -410,12 +436,12 @@ int attn_mask_bits(const AttnMaskArgs& a, hipStream_t st) {
   return hipGetLastError() == hipSuccess ? 0 : 3;
 }
 
+// Blocks that share the keys of a row block: enough for two blocks a CU where there are few row blocks, at least four
+// tiles each.
 int attn_splits(int B, int Hkv, int M, int Sk) {
-  if (M > 32) return 1;
-  const int64_t blocks = (int64_t)B * Hkv;
-  const int tiles = (Sk + 127) / 128;
-  const int64_t want = (1024 + blocks - 1) / blocks;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(want, tiles / 2));
+  const int64_t blocks = (int64_t)((M + 127) / 128) * B * Hkv;
+  const int tiles = M <= FEW_ROWS ? (Sk + 127) / 128 : (Sk + 63) / 64;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(512 / blocks, tiles / 4));
 }
 
 int attn_fwd(const AttnParams& p, hipStream_t st) {

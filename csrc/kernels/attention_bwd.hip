@@ -5,8 +5,12 @@
 // head that shares the key head, so their sum needs no join). The scores and dp are computed in both: 7 products
 // instead of the 5 of a single pass, and in exchange no gradient is summed by atomics: results do not depend on the
 // order in which blocks run, and nothing but the gradients is written.
+// delta is taken from the output before its rounding (o + what that took away): with few keys dp - delta cancels, and a
+// rounded o would leave its whole step there.
 // Rounding: P and dS are rounded to the inputs' type as operands of the second products; everything else is fp32 until
 // the gradients are rounded once.
+#include <algorithm>
+
 #include "attention.h"
 
 namespace {
@@ -14,21 +18,24 @@ namespace {
 using namespace attn;
 
 // dq: QT 32-row tiles per wave, 4 waves along the rows, tiles of KT keys
-template <class T, int DP, int QT, bool MASK>
-__global__ __launch_bounds__(256) void attn_dq_kernel(const AttnParams p) {
+template <class T, int DP, int QT, int KIND>
+__global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
   constexpr int NT = 256, KT = 64, TILE = KT * DP, CPR = DP / 8, CH = KT * CPR / NT;
+  static_assert(KT * CPR % NT == 0, "whole DMA instructions");
   constexpr int NK = KT / 32, NKK = DP / 16, ND = DP / 32, BR = 128 * QT;
+  constexpr bool MASK = KIND == ATTN_MASK;
+  const bool causal = KIND == ATTN_CAUSAL || (MASK && p.causal);
   __shared__ __attribute__((aligned(1024))) bf16_t smem[4 * TILE];
 
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, h = lane >> 5;
-  const int nrb = (p.M + BR - 1) / BR;
-  const int lin = xcd_swizzle(blockIdx.x, gridDim.x);
-  const int bh = lin / nrb, rb0 = lin - bh * nrb;
-  const int rb = p.causal ? nrb - 1 - rb0 : rb0;
+  const int nrb = (p.M + BR - 1) / BR, bhn = p.B * p.Hkv;
+  int rb0, bh, sp;
+  locate(p, nrb, bhn, p.splits, rb0, bh, sp);
+  const int rb = causal ? nrb - 1 - rb0 : rb0;
   const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const int len = p.lengths ? imin(imax(p.lengths[b], 0), p.Sk) : p.Sk;
-  const int off = p.causal ? p.Sk - p.Sq : 0;
+  const int off = causal ? p.Sk - p.Sq : 0;
 
   s8v qf[QT][NKK], gf[QT][NKK];
   int lim[QT], ri[QT], rg[QT];
@@ -42,37 +49,41 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(const AttnParams p) {
     rg[t] = g;
     lse[t] = p.lse2[(int64_t)bh * p.M + rr];
     const bool use = ok && lse[t] != INFINITY;            // an empty row takes part in nothing, whatever it holds
-    lim[t] = !use ? 0 : p.causal ? imin(imax(i + off + 1, 0), len) : len;
+    lim[t] = !use ? 0 : causal ? imin(imax(i + off + 1, 0), len) : len;
     const bf16_t* q = reinterpret_cast<const bf16_t*>(p.q.p) + b * p.q.sb + i * p.q.ss + (hk * p.G + g) * p.q.sh;
     const bf16_t* go = reinterpret_cast<const bf16_t*>(p.go.p) + b * p.go.sb + i * p.go.ss + (hk * p.G + g) * p.go.sh;
-    const bf16_t* o = reinterpret_cast<const bf16_t*>(p.o.p) + b * p.o.sb + i * p.o.ss + (hk * p.G + g) * p.o.sh;
+    const int64_t at = b * p.o.sb + i * p.o.ss + (hk * p.G + g) * p.o.sh;
+    const bf16_t *o = reinterpret_cast<const bf16_t*>(p.o.p) + at, *rest = p.o_rest + at;
     float dl = 0.f;
 #pragma unroll
     for (int kk = 0; kk < NKK; ++kk) {
       const int d = 16 * kk + 8 * h;
-      u4v wq = {0, 0, 0, 0}, wg = wq, wo = wq;
+      u4v wq = {0, 0, 0, 0}, wg = wq, wo = wq, wr = wq;
       if (use && d < p.D) {
         wq = *reinterpret_cast<const u4v*>(q + d);
         wg = *reinterpret_cast<const u4v*>(go + d);
         wo = *reinterpret_cast<const u4v*>(o + d);
+        wr = *reinterpret_cast<const u4v*>(rest + d);
       }
 #pragma unroll
-      for (int x = 0; x < 4; ++x) dl = fmaf(T::lo(wg[x]), T::lo(wo[x]), fmaf(T::hi(wg[x]), T::hi(wo[x]), dl));
+      for (int x = 0; x < 4; ++x)
+        dl = fmaf(T::lo(wg[x]), T::lo(wo[x]) + T::lo(wr[x]), fmaf(T::hi(wg[x]), T::hi(wo[x]) + T::hi(wr[x]), dl));
       qf[t][kk] = __builtin_bit_cast(s8v, wq);
       gf[t][kk] = __builtin_bit_cast(s8v, wg);
     }
     delta[t] = dl + other_half(dl);
-    if (ok && h == 0) p.delta[(int64_t)bh * p.M + r] = delta[t];
+    if (ok && h == 0 && sp == 0) p.delta[(int64_t)bh * p.M + r] = delta[t];
   }
   if (p.dq.p == nullptr) return;
 
   const int r_end = imin(rb * BR + BR, p.M), i_last = fdiv(r_end - 1, p.div_g);
-  const int kend = p.causal ? imin(imax(i_last + off + 1, 0), len) : len;
+  const int kend = causal ? imin(imax(i_last + off + 1, 0), len) : len;
   const int wr0 = rb * BR + wid * QT * 32;
   const int wi0 = fdiv(imin(wr0, p.M - 1), p.div_g), wi1 = fdiv(imin(wr0 + QT * 32, p.M) - 1, p.div_g);
-  const int wlast = wr0 >= p.M ? 0 : p.causal ? imin(imax(wi1 + off + 1, 0), len) : len;
-  const int wfull = p.causal ? imin(imax(wi0 + off + 1, 0), len) : len;
-  const int tiles = (p.Sk + KT - 1) / KT, t1 = (kend + KT - 1) / KT;
+  const int wlast = wr0 >= p.M ? 0 : causal ? imin(imax(wi1 + off + 1, 0), len) : len;
+  const int wfull = causal ? imin(imax(wi0 + off + 1, 0), len) : len;
+  const int tiles = (p.Sk + KT - 1) / KT, tps = (tiles + p.splits - 1) / p.splits;
+  const int t0 = sp * tps, t1 = imin(imin(t0 + tps, tiles), (kend + KT - 1) / KT);
 
   uint32_t vk[CH], vv[CH];
   int vrow[CH];
@@ -104,136 +115,186 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(const AttnParams p) {
       mrow[t] = p.mask.bits + (b * p.mask.sb + (hk * p.G + rg[t]) * p.mask.sh + (p.mask.rows > 1 ? ri[t] : 0)) *
                                   (int64_t)p.mask.words;
   }
+  __shared__ uint8_t classes[MASK ? MASK_TILES + 64 : 1];
   TileMask tm;
-  if (MASK) tm.init(p, b, hk);
-  const int ib0 = fdiv(rb * BR, p.div_g), ib1 = i_last;
-  auto next = [&](int t) {
-    if (!MASK) return t;
-    return tm.next(t, t1, [&](int u) { return tm.cls(p, ib0, ib1, u, u, u < tiles); });
-  };
+  if (MASK)
+    tm.fill(p, b, hk, classes, tiles, [&](int t, int& i0, int& i1, int& w0, int& w1) {
+      i0 = fdiv(rb * BR, p.div_g);
+      i1 = i_last;
+      w0 = w1 = t;
+    });
+  auto next = [&](int t) { return MASK ? tm.next(t, t1) : t; };
   auto words = [&](int t) {
 #pragma unroll
     for (int u = 0; u < QT; ++u) word[u] = mrow[u][imin(t, p.mask.words - 1)];
   };
 
   f16v acc[ND][QT];
-#pragma unroll
-  for (int d = 0; d < ND; ++d)
-#pragma unroll
-    for (int t = 0; t < QT; ++t)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[d][t][e] = 0.f;
   const float sc = p.scale * LOG2E;
+  auto walk = [&](auto safe) {
+    constexpr bool SAFE = decltype(safe)::value;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[d][t][e] = 0.f;
 
-  int t = next(0), buf = 0;
-  if (t < t1) {
-    if (MASK) words(t);
-    issue(t, 0);
-  }
-  wait_vm();
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-  while (t < t1) {
-    const int key0 = t * KT;
-    const bool part = MASK && !tm.is_whole(t);
-    const int tn = next(t + 1);
-    unsigned long long cur[QT];
-    if (MASK) {
-#pragma unroll
-      for (int u = 0; u < QT; ++u) cur[u] = word[u];
-      if (tn < t1) words(tn);
+    int t = next(t0), buf = 0;
+    if (t < t1) {
+      if (MASK) words(t);
+      issue(t, 0);
     }
-    if (tn < t1) issue(tn, buf ^ 1);
-    if (key0 < wlast) {
-      const bf16_t* sk = smem + buf * 2 * TILE;
-      const bf16_t* sv = sk + TILE;
-      const bool edge = key0 + KT > wfull;
-#pragma unroll
-      for (int k = 0; k < NK; ++k) {
-        f16v s[QT], dp[QT];
-#pragma unroll
-        for (int u = 0; u < QT; ++u)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) s[u][e] = dp[u][e] = 0.f;
-#pragma unroll
-        for (int kk = 0; kk < NKK; ++kk) {
-          const s8v a = frag<DP>(sk, 32 * k + c, 2 * kk + h);
-#pragma unroll
-          for (int u = 0; u < QT; ++u) s[u] = T::mma(a, qf[u][kk], s[u]);
-        }
-#pragma unroll
-        for (int kk = 0; kk < NKK; ++kk) {
-          const s8v a = frag<DP>(sv, 32 * k + c, 2 * kk + h);
-#pragma unroll
-          for (int u = 0; u < QT; ++u) dp[u] = T::mma(a, gf[u][kk], dp[u]);
-        }
-        s8v db[QT][2];
-#pragma unroll
-        for (int u = 0; u < QT; ++u) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) s[u][e] = exp2_(fmaf(s[u][e], sc, -lse[u])) * (dp[u][e] - delta[u]);
-          if (MASK && part) {
-            const uint32_t w = (uint32_t)(cur[u] >> (32 * k)) >> (4 * h);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[u][e] = (w >> ((e & 3) + 8 * (e >> 2))) & 1 ? s[u][e] : 0.f;
-          }
-          if (edge) {
-            const int left = lim[u] - key0 - 32 * k - 4 * h;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[u][e] = (e & 3) + 8 * (e >> 2) < left ? s[u][e] : 0.f;
-          }
-          db[u][0] = pack_b<T>(s[u], 0);
-          db[u][1] = pack_b<T>(s[u], 1);
-        }
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-          for (int d = 0; d < ND; ++d) {
-            const s8v a = frag_t<DP>(sk, 32 * k + 16 * ks, d, lane);
-#pragma unroll
-            for (int u = 0; u < QT; ++u) acc[d][u] = T::mma(a, db[u][ks], acc[d][u]);
-          }
-      }
-    }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    wait_vm();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    buf ^= 1;
-    t = tn;
+    while (t < t1) {
+      const int key0 = t * KT;
+      const bool part = MASK && tm.part;
+      const int tn = next(t + 1);
+      unsigned long long cur[QT];
+      if (MASK) {
+#pragma unroll
+        for (int u = 0; u < QT; ++u) cur[u] = word[u];
+        if (tn < t1) words(tn);
+      }
+      if (tn < t1) issue(tn, buf ^ 1);
+      if (key0 < wlast) {
+        const bf16_t* sk = smem + buf * 2 * TILE;
+        const bf16_t* sv = sk + TILE;
+        const bool edge = key0 + KT > wfull;
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+          f16v s[QT], dp[QT];
+          // 128 channels: fragment addresses are formed at each read from one offset that the compiler must not see
+          // through, or it keeps all of them in registers that are not there
+          int fo = lds_at<DP>(c, h);
+          if (DP == 128) asm volatile("" : "+v"(fo));
+          float nd[QT];
+#pragma unroll
+          for (int u = 0; u < QT; ++u) {
+            nd[u] = -delta[u];
+            asm volatile("" : "+v"(nd[u]));                // or 16 copies of it stay in registers
+          }
+#pragma unroll
+          for (int u = 0; u < QT; ++u)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              s[u][e] = 0.f;
+              dp[u][e] = nd[u];                            // the product sums dp - delta
+            }
+#pragma unroll
+          for (int kk = 0; kk < NKK; ++kk) {
+            const s8v a = frag_x<DP>(sk + 32 * k * DP, fo, kk);
+#pragma unroll
+            for (int u = 0; u < QT; ++u) s[u] = T::mma(a, qf[u][kk], s[u]);
+          }
+#pragma unroll
+          for (int kk = 0; kk < NKK; ++kk) {
+            const s8v a = frag_x<DP>(sv + 32 * k * DP, fo, kk);
+#pragma unroll
+            for (int u = 0; u < QT; ++u) dp[u] = T::mma(a, gf[u][kk], dp[u]);
+          }
+          s8v db[QT][2];
+          if (DP == 128) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int u = 0; u < QT; ++u) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[u][e] = exp2_(fmaf(s[u][e], sc, -lse[u]));
+            if (MASK && part) {
+              const uint32_t w = (uint32_t)(cur[u] >> (32 * k)) >> (4 * h);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) s[u][e] = (w >> ((e & 3) + 8 * (e >> 2))) & 1 ? s[u][e] : 0.f;
+            }
+            if (edge) {
+              const int left = lim[u] - key0 - 32 * k - 4 * h;
+#pragma unroll
+              for (int e = 0; e < 16; ++e) s[u][e] = (e & 3) + 8 * (e >> 2) < left ? s[u][e] : 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float ds = s[u][e] * dp[u][e];
+              s[u][e] = SAFE && s[u][e] == 0.f ? 0.f : ds;
+            }
+            db[u][0] = pack_b<T>(s[u], 0);
+            db[u][1] = pack_b<T>(s[u], 1);
+          }
+          if (DP == 128) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+              s8v a = frag_t<DP>(sk, 32 * k + 16 * ks, d, lane);
+              if constexpr (SAFE) {                          // an allowed key that is not finite shows in its scores
+                s8v pos, neg;
+                __builtin_amdgcn_sched_barrier(0);         // few registers matter here, not speed
+                a = clean<T>(a, pos, neg);
+              }
+#pragma unroll
+              for (int u = 0; u < QT; ++u) acc[d][u] = T::mma(a, db[u][ks], acc[d][u]);
+            }
+        }
+      }
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      buf ^= 1;
+      t = tn;
+    }
+  };
+  walk(std::false_type{});
+  if constexpr (KIND != ATTN_PLAIN) {
+    float z = 0.f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int u = 0; u < QT; ++u) z += finite_sum(acc[d][u]);
+    if (__syncthreads_or(z != 0.f)) walk(std::true_type{});
   }
 #pragma unroll
   for (int u = 0; u < QT; ++u) {
     const bool ok = rb * BR + (wid * QT + u) * 32 + c < p.M;
+    if (p.splits > 1) {
+      const int64_t part = ((int64_t)sp * bhn + bh) * p.M + rb * BR + (wid * QT + u) * 32 + c;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) store_part<DP>(p.ws_o + part * DP, acc[d][u], p.scale, d, h, ok);
+      continue;
+    }
     bf16_t* o = reinterpret_cast<bf16_t*>(p.dq.p) + b * p.dq.sb + ri[u] * p.dq.ss + (hk * p.G + rg[u]) * p.dq.sh;
 #pragma unroll
     for (int d = 0; d < ND; ++d) store_row<T>(o, acc[d][u], p.scale, d, p.D, h, ok);
   }
 }
 
-// dk, dv: KQ 32-key tiles per wave, 4 waves along the keys, tiles of RT rows
-template <class T, int DP, int KQ, bool MASK>
-__global__ __launch_bounds__(256) void attn_dkv_kernel(const AttnParams p) {
-  constexpr int NT = 256, RT = 64, TILE = RT * DP, CPR = DP / 8, CH = RT * CPR / NT;
+// dk, dv: KQ 32-key tiles per wave, 4 waves along the keys, tiles of RT rows. The wave's keys are B operands in registers
+// for the whole walk, its values too, or (VL: from 96 channels, where dk and dv take half of the 256 registers that let
+// two waves share a SIMD) in LDS.
+template <class T, int DP, int KQ, int RT, bool VL, int KIND>
+__global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
+  constexpr int NT = 256, TILE = RT * DP, CPR = DP / 8, CH = RT * CPR / NT, VTILE = VL ? 128 * KQ * DP : 0;
+  static_assert(RT * CPR % NT == 0 && VTILE / 8 % NT == 0, "whole DMA instructions");
   constexpr int NR = RT / 32, NKK = DP / 16, ND = DP / 32, BK = 128 * KQ;
-  __shared__ __attribute__((aligned(1024))) bf16_t smem[4 * TILE];
-  __shared__ __attribute__((aligned(256))) float sstat[2][2][RT];      // [buffer][lse2, delta][row]
+  constexpr bool MASK = KIND == ATTN_MASK;
+  const bool causal = KIND == ATTN_CAUSAL || (MASK && p.causal);
+  __shared__ __attribute__((aligned(1024))) bf16_t smem[4 * TILE + VTILE];
+  __shared__ __attribute__((aligned(256))) float sstat[2][2][64];      // [buffer][lse2, delta][row]
 
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, h = lane >> 5;
-  const int nkb = (p.Sk + BK - 1) / BK;
-  const int lin = xcd_swizzle(blockIdx.x, gridDim.x);
-  const int bh = lin / nkb, kb = lin - bh * nkb;            // causal: the first keys have the most rows
+  const int nkb = (p.Sk + BK - 1) / BK, bhn = p.B * p.Hkv;
+  int kb, bh, sp;
+  locate(p, nkb, bhn, p.kv_splits, kb, bh, sp);             // causal: the first keys have the most rows
   const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const int len = p.lengths ? imin(imax(p.lengths[b], 0), p.Sk) : p.Sk;
-  const int off = p.causal ? p.Sk - p.Sq : 0;
+  const int off = causal ? p.Sk - p.Sq : 0;
   const int wkey0 = kb * BK + wid * KQ * 32;
 
-  s8v kf[KQ][NKK], vf[KQ][NKK];
+  s8v kf[KQ][NKK], vf[KQ][VL ? 1 : NKK];
   int rmin[KQ];                                              // first row that may attend this lane's key
 #pragma unroll
   for (int t = 0; t < KQ; ++t) {
     const int key = wkey0 + 32 * t + c;
-    rmin[t] = p.causal ? imin(imax(key - off, 0), p.Sq) * p.G : 0;
+    rmin[t] = causal ? imin(imax(key - off, 0), p.Sq) * p.G : 0;
     const bf16_t* k = reinterpret_cast<const bf16_t*>(p.k.p) + b * p.k.sb + key * p.k.ss + hk * p.k.sh;
     const bf16_t* v = reinterpret_cast<const bf16_t*>(p.v.p) + b * p.v.sb + key * p.v.ss + hk * p.v.sh;
 #pragma unroll
@@ -242,19 +303,30 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(const AttnParams p) {
       u4v wk = {0, 0, 0, 0}, wv = wk;
       if (key < len && d < p.D) {
         wk = *reinterpret_cast<const u4v*>(k + d);
-        wv = *reinterpret_cast<const u4v*>(v + d);
+        if (!VL) wv = *reinterpret_cast<const u4v*>(v + d);
       }
       kf[t][kk] = __builtin_bit_cast(s8v, wk);
-      vf[t][kk] = __builtin_bit_cast(s8v, wv);
+      if (!VL) vf[t][VL ? 0 : kk] = __builtin_bit_cast(s8v, wv);
+    }
+  }
+  const bf16_t* svals = smem + 4 * TILE + wid * KQ * 32 * DP;
+  if (VL) {
+    const u4v rv = rsrc(reinterpret_cast<const bf16_t*>(p.v.p) + b * p.v.sb + (int64_t)kb * BK * p.v.ss + hk * p.v.sh);
+#pragma unroll
+    for (int n = 0; n < VTILE / 8 / NT; ++n) {
+      const int id = tid + NT * n, row = id / CPR, d = ((id % CPR) ^ swz<DP>(row)) * 8;
+      dma16(rv, kb * BK + row < len && d < p.D ? (uint32_t)(row * (int)p.v.ss + d) * 2 : CFL_OOB,
+            smem + 4 * TILE + wid * 512 + NT * 8 * n);
     }
   }
   const int klast = imin(kb * BK + BK, p.Sk) - 1;
   const int tiles = (p.M + RT - 1) / RT;
-  const int t0 = p.causal ? imin(imax(kb * BK - off, 0), p.Sq) * p.G / RT : 0;
-  const int t1 = kb * BK < len ? tiles : 0;
+  const int tfirst = causal ? imin(imax(kb * BK - off, 0), p.Sq) * p.G / RT : 0;
+  const int tps = (tiles - tfirst + p.kv_splits - 1) / p.kv_splits;      // the walk's own tiles in even parts
+  const int t0 = tfirst + sp * tps, t1 = kb * BK < len ? imin(t0 + tps, tiles) : 0;
   // rows below wfirst attend no key of this wave, rows from wfull on every one
-  const int wfirst = p.causal ? imin(imax(wkey0 - off, 0), p.Sq) * p.G : 0;
-  const int wfull = p.causal ? imin(imax(imin(wkey0 + 32 * KQ, p.Sk) - 1 - off, 0), p.Sq) * p.G : 0;
+  const int wfirst = causal ? imin(imax(wkey0 - off, 0), p.Sq) * p.G : 0;
+  const int wfull = causal ? imin(imax(imin(wkey0 + 32 * KQ, p.Sk) - 1 - off, 0), p.Sq) * p.G : 0;
 
   int vrow[CH], vd[CH];
 #pragma unroll
@@ -281,20 +353,20 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(const AttnParams p) {
     // rows past the last read 0 everywhere: p = 1, do = 0, ds = 0
     if (wid < 2) {
       const u4v rs = rsrc((wid ? p.delta : p.lse2) + (int64_t)bh * p.M + r0);
-      dma4(rs, lane < rem ? 4u * lane : CFL_OOB, &sstat[buf][wid][0]);
+      dma4(rs, lane < imin(rem, RT) ? 4u * lane : CFL_OOB, &sstat[buf][wid][0]);
     }
   };
 
+  __shared__ uint8_t classes[MASK ? MASK_TILES + 64 : 1];
   TileMask tm;
-  if (MASK) tm.init(p, b, hk);
-  auto next = [&](int t) {
-    if (!MASK) return t;
-    return tm.next(t, t1, [&](int u) {
-      const int last = imin(u * RT + RT, p.M) - 1;
-      return tm.cls(p, fdiv(imin(u * RT, p.M - 1), p.div_g), fdiv(imax(last, 0), p.div_g), kb * BK >> 6, klast >> 6,
-                    u < tiles);
+  if (MASK)
+    tm.fill(p, b, hk, classes, tiles, [&](int t, int& i0, int& i1, int& w0, int& w1) {
+      i0 = fdiv(t * RT, p.div_g);
+      i1 = fdiv(imin(t * RT + RT, p.M) - 1, p.div_g);
+      w0 = kb * BK >> 6;
+      w1 = klast >> 6;
     });
-  };
+  auto next = [&](int t) { return MASK ? tm.next(t, t1) : t; };
   // mask bits of row 32 * n + c of the tile against the wave's keys
   uint32_t bits[NR][KQ], cur[NR][KQ];
   auto words = [&](int t) {
@@ -313,120 +385,152 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(const AttnParams p) {
   };
 
   f16v dk[ND][KQ], dv[ND][KQ];
-#pragma unroll
-  for (int d = 0; d < ND; ++d)
-#pragma unroll
-    for (int u = 0; u < KQ; ++u)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) dk[d][u][e] = dv[d][u][e] = 0.f;
   const float sc = p.scale * LOG2E;
-
-  int t = t1 > t0 ? next(t0) : t0, buf = 0;
-  if (t < t1) {
-    if (MASK) words(t);
-    issue(t, 0);
-  }
-  wait_vm();
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-  while (t < t1) {
-    const bool part = MASK && !tm.is_whole(t);
-    const int tn = next(t + 1);
-    if (MASK) {
+  auto walk = [&](auto safe) {
+    constexpr bool SAFE = decltype(safe)::value;
 #pragma unroll
-      for (int n = 0; n < NR; ++n)
-#pragma unroll
-        for (int u = 0; u < KQ; ++u) cur[n][u] = bits[n][u];
-      if (tn < t1) words(tn);
-    }
-    if (tn < t1) issue(tn, buf ^ 1);
-    const bf16_t* sq = smem + buf * 2 * TILE;
-    const bf16_t* sg = sq + TILE;
-#pragma unroll
-    for (int n = 0; n < NR; ++n) {
-      const int r0 = t * RT + 32 * n;
-      if (r0 + 32 <= wfirst || r0 >= p.M || wkey0 >= len) continue;
-      const bool edge = r0 < wfull;
-      f16v s[KQ], dp[KQ];
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int u = 0; u < KQ; ++u)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[u][e] = dp[u][e] = 0.f;
-#pragma unroll
-      for (int kk = 0; kk < NKK; ++kk) {
-        const s8v a = frag<DP>(sq, 32 * n + c, 2 * kk + h);
-#pragma unroll
-        for (int u = 0; u < KQ; ++u) s[u] = T::mma(a, kf[u][kk], s[u]);
-      }
-#pragma unroll
-      for (int kk = 0; kk < NKK; ++kk) {
-        const s8v a = frag<DP>(sg, 32 * n + c, 2 * kk + h);
-#pragma unroll
-        for (int u = 0; u < KQ; ++u) dp[u] = T::mma(a, vf[u][kk], dp[u]);
-      }
-      float lse[16], dl[16];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float4 x = *reinterpret_cast<const float4*>(&sstat[buf][0][32 * n + 8 * q + 4 * h]);
-        const float4 y = *reinterpret_cast<const float4*>(&sstat[buf][1][32 * n + 8 * q + 4 * h]);
-        lse[4 * q] = x.x; lse[4 * q + 1] = x.y; lse[4 * q + 2] = x.z; lse[4 * q + 3] = x.w;
-        dl[4 * q] = y.x; dl[4 * q + 1] = y.y; dl[4 * q + 2] = y.z; dl[4 * q + 3] = y.w;
-      }
-      s8v pb[KQ][2], db[KQ][2];
-#pragma unroll
-      for (int u = 0; u < KQ; ++u) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          s[u][e] = exp2_(fmaf(s[u][e], sc, -lse[e]));
-          dp[u][e] = s[u][e] * (dp[u][e] - dl[e]);
-        }
-        if (MASK && part) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int row = (e & 3) + 8 * (e >> 2);
-            const uint32_t lo = __builtin_amdgcn_readlane(cur[n][u], row);
-            const uint32_t hi = __builtin_amdgcn_readlane(cur[n][u], row + 4);
-            const bool ok = __builtin_amdgcn_inverse_ballot_w64(((unsigned long long)hi << 32) | lo);
-            s[u][e] = ok ? s[u][e] : 0.f;
-            dp[u][e] = ok ? dp[u][e] : 0.f;
-          }
-        }
-        if (edge) {
-          const int from = rmin[u] - r0 - 4 * h;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const bool ok = (e & 3) + 8 * (e >> 2) >= from;
-            s[u][e] = ok ? s[u][e] : 0.f;
-            dp[u][e] = ok ? dp[u][e] : 0.f;
-          }
-        }
-        pb[u][0] = pack_b<T>(s[u], 0);
-        pb[u][1] = pack_b<T>(s[u], 1);
-        db[u][0] = pack_b<T>(dp[u], 0);
-        db[u][1] = pack_b<T>(dp[u], 1);
-      }
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          const s8v a = frag_t<DP>(sg, 32 * n + 16 * ks, d, lane);
-#pragma unroll
-          for (int u = 0; u < KQ; ++u) dv[d][u] = T::mma(a, pb[u][ks], dv[d][u]);
-        }
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          const s8v a = frag_t<DP>(sq, 32 * n + 16 * ks, d, lane);
-#pragma unroll
-          for (int u = 0; u < KQ; ++u) dk[d][u] = T::mma(a, db[u][ks], dk[d][u]);
-        }
+        for (int e = 0; e < 16; ++e) dk[d][u][e] = dv[d][u][e] = 0.f;
+
+    int t = t1 > t0 ? next(t0) : t0, buf = 0;
+    if (t < t1) {
+      if (MASK) words(t);
+      issue(t, 0);
     }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    wait_vm();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    buf ^= 1;
-    t = tn;
+    while (t < t1) {
+      const bool part = MASK && tm.part;
+      const int tn = next(t + 1);
+      if (MASK) {
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+          for (int u = 0; u < KQ; ++u) cur[n][u] = bits[n][u];
+        if (tn < t1) words(tn);
+      }
+      if (tn < t1) issue(tn, buf ^ 1);
+      const bf16_t* sq = smem + buf * 2 * TILE;
+      const bf16_t* sg = sq + TILE;
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        const int r0 = t * RT + 32 * n;
+        if (r0 + 32 <= wfirst || r0 >= p.M || wkey0 >= len) continue;
+        const bool edge = r0 < wfull;
+        // VL: addresses from one offset, as in attn_dq_kernel
+        int fo = lds_at<DP>(c, h);
+        if (VL) asm volatile("" : "+v"(fo));
+        f16v s[KQ], dp[KQ];
+        if (VL) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < KQ; ++u)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f4v y = *reinterpret_cast<const f4v*>(&sstat[buf][1][32 * n + 8 * q + 4 * h]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              s[u][4 * q + j] = 0.f;
+              dp[u][4 * q + j] = -y[j];                    // the product sums dp - delta
+            }
+          }
+#pragma unroll
+        for (int kk = 0; kk < NKK; ++kk) {
+          const s8v a = frag_x<DP>(sq + 32 * n * DP, fo, kk);
+#pragma unroll
+          for (int u = 0; u < KQ; ++u) s[u] = T::mma(a, kf[u][kk], s[u]);
+          if (VL && kk % 8 == 7) __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int kk = 0; kk < NKK; ++kk) {
+          const s8v a = frag_x<DP>(sg + 32 * n * DP, fo, kk);
+#pragma unroll
+          for (int u = 0; u < KQ; ++u)
+            dp[u] = T::mma(a, VL ? frag_x<DP>(svals + 32 * u * DP, fo, kk) : vf[u][VL ? 0 : kk], dp[u]);
+          if (VL && kk % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+        s8v pb[KQ][2], db[KQ][2];
+        if (VL) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < KQ; ++u) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f4v x = *reinterpret_cast<const f4v*>(&sstat[buf][0][32 * n + 8 * q + 4 * h]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[u][4 * q + j] = exp2_(fmaf(s[u][4 * q + j], sc, -x[j]));
+          }
+          if (MASK && part) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int row = (e & 3) + 8 * (e >> 2);
+              const uint32_t lo = __builtin_amdgcn_readlane(cur[n][u], row);
+              const uint32_t hi = __builtin_amdgcn_readlane(cur[n][u], row + 4);
+              s[u][e] = __builtin_amdgcn_inverse_ballot_w64(((unsigned long long)hi << 32) | lo) ? s[u][e] : 0.f;
+            }
+          }
+          if (edge) {
+            const int from = rmin[u] - r0 - 4 * h;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[u][e] = (e & 3) + 8 * (e >> 2) >= from ? s[u][e] : 0.f;
+          }
+          pb[u][0] = pack_b<T>(s[u], 0);
+          pb[u][1] = pack_b<T>(s[u], 1);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            dp[u][e] *= s[u][e];
+            if constexpr (SAFE) dp[u][e] = s[u][e] == 0.f ? 0.f : dp[u][e];
+          }
+          db[u][0] = pack_b<T>(dp[u], 0);
+          db[u][1] = pack_b<T>(dp[u], 1);
+        }
+        if (VL) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int d = 0; d < ND; ++d) {
+            s8v a = frag_t<DP>(sg, 32 * n + 16 * ks, d, lane);
+            if constexpr (SAFE) {
+              s8v pos, neg;
+              __builtin_amdgcn_sched_barrier(0);           // few registers matter here, not speed
+              a = clean<T>(a, pos, neg);
+#pragma unroll
+              for (int u = 0; u < KQ; ++u) poison<T>(dv[d][u], pos, neg, pb[u][ks]);
+            }
+#pragma unroll
+            for (int u = 0; u < KQ; ++u) dv[d][u] = T::mma(a, pb[u][ks], dv[d][u]);
+          }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int d = 0; d < ND; ++d) {
+            s8v a = frag_t<DP>(sq, 32 * n + 16 * ks, d, lane);
+            if constexpr (SAFE) {                            // an allowed query that is not finite shows in its scores
+              s8v pos, neg;
+              __builtin_amdgcn_sched_barrier(0);           // few registers matter here, not speed
+              a = clean<T>(a, pos, neg);
+            }
+#pragma unroll
+            for (int u = 0; u < KQ; ++u) dk[d][u] = T::mma(a, db[u][ks], dk[d][u]);
+          }
+      }
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      buf ^= 1;
+      t = tn;
+    }
+  };
+  walk(std::false_type{});
+  if constexpr (KIND != ATTN_PLAIN) {
+    float z = 0.f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int u = 0; u < KQ; ++u) z += finite_sum(dk[d][u]) + finite_sum(dv[d][u]);
+    if (__syncthreads_or(z != 0.f)) walk(std::true_type{});
   }
 #pragma unroll
   for (int u = 0; u < KQ; ++u) {
@@ -439,6 +543,15 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(const AttnParams p) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) dk[d][u][e] = dv[d][u][e] = 0.f;
     }
+    if (p.kv_splits > 1) {
+      const int64_t part = ((int64_t)sp * bhn + bh) * p.Sk + key, half = (int64_t)p.kv_splits * bhn * p.Sk;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        store_part<DP>(p.ws_kv + part * DP, dk[d][u], p.scale, d, h, key < p.Sk);
+        store_part<DP>(p.ws_kv + (half + part) * DP, dv[d][u], 1.f, d, h, key < p.Sk);
+      }
+      continue;
+    }
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
       if (p.dk.p) store_row<T>(ko, dk[d][u], p.scale, d, p.D, h, key < p.Sk);
@@ -447,35 +560,75 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(const AttnParams p) {
   }
 }
 
-template <class T, int DP, bool MASK>
-void bwd(const AttnParams& p, hipStream_t st) {
-  const unsigned nq = (unsigned)((p.M + 127) / 128 * (int64_t)p.B * p.Hkv);
-  attn_dq_kernel<T, DP, 1, MASK><<<nq, 256, 0, st>>>(p);
-  if (p.dk.p == nullptr && p.dv.p == nullptr) return;
-  const unsigned nk = (unsigned)((p.Sk + 127) / 128 * (int64_t)p.B * p.Hkv);
-  if (nk) attn_dkv_kernel<T, DP, 1, MASK><<<nk, 256, 0, st>>>(p);
+// gradients of a token tensor from the parts of `splits` blocks: one thread per 4 channels, parts in order
+template <class T, int DP>
+__global__ __launch_bounds__(256) void attn_sum_kernel(const float* ws, int splits, AttnTensor out, int B, int H, int G,
+                                                       int rows, int D, FastDiv div_g) {
+  constexpr int TPR = DP / 4;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (int64_t)B * H * rows, row = id / TPR;
+  const int d = (int)(id % TPR) * 4;
+  if (row >= all || d >= D) return;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < splits; ++s) {
+    const float4 v = *reinterpret_cast<const float4*>(ws + (s * all + row) * DP + d);
+    a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+  }
+  const int bh = (int)(row / rows), r = (int)(row - (int64_t)bh * rows), b = bh / H, hk = bh - b * H;
+  const int i = fdiv(r, div_g), g = r - i * G;
+  bf16_t* o = reinterpret_cast<bf16_t*>(out.p) + b * out.sb + i * out.ss + (hk * G + g) * out.sh + d;
+  *reinterpret_cast<uint2*>(o) = make_uint2(T::pack2(a.x, a.y), T::pack2(a.z, a.w));
 }
 
-template <class T, bool MASK>
+template <class T, int DP, int KIND>
+void bwd(const AttnParams& p, hipStream_t st) {
+  const int64_t bhn = (int64_t)p.B * p.Hkv;
+  attn_dq_kernel<T, DP, 1, KIND><<<(unsigned)((p.M + 127) / 128 * bhn * p.splits), 256, 0, st>>>(p);
+  if (p.splits > 1 && p.dq.p)
+    attn_sum_kernel<T, DP><<<(unsigned)((bhn * p.M * (DP / 4) + 255) / 256), 256, 0, st>>>(
+        p.ws_o, p.splits, p.dq, p.B, p.Hkv, p.G, p.M, p.D, p.div_g);
+  if ((p.dk.p == nullptr && p.dv.p == nullptr) || p.Sk == 0) return;
+  constexpr bool VL = DP >= 96;
+  attn_dkv_kernel<T, DP, 1, DP == 128 ? 32 : 64, VL, KIND>
+      <<<(unsigned)((p.Sk + 127) / 128 * bhn * p.kv_splits), 256, 0, st>>>(p);
+  if (p.kv_splits > 1) {
+    const int64_t n = bhn * p.Sk;
+    const unsigned grid = (unsigned)((n * (DP / 4) + 255) / 256);
+    const FastDiv one = fast_div(1);
+    if (p.dk.p)
+      attn_sum_kernel<T, DP><<<grid, 256, 0, st>>>(p.ws_kv, p.kv_splits, p.dk, p.B, p.Hkv, 1, p.Sk, p.D, one);
+    if (p.dv.p)
+      attn_sum_kernel<T, DP><<<grid, 256, 0, st>>>(p.ws_kv + p.kv_splits * n * DP, p.kv_splits, p.dv, p.B, p.Hkv, 1,
+                                                   p.Sk, p.D, one);
+  }
+}
+
+template <class T, int KIND>
 void bwd_d(const AttnParams& p, hipStream_t st) {
-  if (p.D <= 32) bwd<T, 32, MASK>(p, st);
-  else if (p.D <= 64) bwd<T, 64, MASK>(p, st);
-  else if (p.D <= 96) bwd<T, 96, MASK>(p, st);
-  else bwd<T, 128, MASK>(p, st);
+  if (p.D <= 32) bwd<T, 32, KIND>(p, st);
+  else if (p.D <= 64) bwd<T, 64, KIND>(p, st);
+  else if (p.D <= 96) bwd<T, 96, KIND>(p, st);
+  else bwd<T, 128, KIND>(p, st);
 }
 
 }  // namespace
 
+// Blocks that share a row block's keys (dq) and a key block's rows (dk, dv): as attn_splits, up to two blocks a CU, or
+// four for causal dk, dv, whose blocks are as unequal as their keys (2 images, 16 heads that share 2, 8,192 tokens, 128
+// channels: 2,862 / 2,041 / 2,053 us for 512 / 1,024 / 2,048 blocks); at least four tiles each.
+void attn_bwd_splits(int B, int Hkv, int M, int Sk, int causal, int& splits, int& kv_splits) {
+  const int64_t bhn = (int64_t)B * Hkv, qb = (M + 127) / 128 * bhn, kb = std::max<int64_t>(1, (Sk + 127) / 128 * bhn);
+  splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / qb, (Sk + 63) / 64 / 4));
+  kv_splits = (int)std::max<int64_t>(1, std::min<int64_t>((causal ? 1024 : 512) / kb, (M + 63) / 64 / 4));
+}
+
 int attn_bwd(const AttnParams& p, hipStream_t st) {
-  if (p.D < 8 || p.D > 128 || p.D % 8 || p.M < 1 || p.Sk < 0) return 1;
-  if ((p.M + 127) / 128 * (int64_t)p.B * p.Hkv > 0x7fffffff || (p.Sk + 127) / 128 * (int64_t)p.B * p.Hkv > 0x7fffffff)
+  if (p.D < 8 || p.D > 128 || p.D % 8 || p.M < 1 || p.Sk < 0 || p.splits < 1 || p.kv_splits < 1) return 1;
+  if ((p.M + 127) / 128 * (int64_t)p.B * p.Hkv * p.splits > 0x7fffffff ||
+      (p.Sk + 127) / 128 * (int64_t)p.B * p.Hkv * p.kv_splits > 0x7fffffff)
     return 2;
-  if (p.mask.bits) {
-    if (p.fp16) bwd_d<FP16, true>(p, st);
-    else bwd_d<BF16, true>(p, st);
-  } else {
-    if (p.fp16) bwd_d<FP16, false>(p, st);
-    else bwd_d<BF16, false>(p, st);
-  }
+  const int kind = p.mask.bits ? ATTN_MASK : p.causal ? ATTN_CAUSAL : ATTN_PLAIN;
+  if (kind == ATTN_MASK) p.fp16 ? bwd_d<FP16, ATTN_MASK>(p, st) : bwd_d<BF16, ATTN_MASK>(p, st);
+  else if (kind == ATTN_CAUSAL) p.fp16 ? bwd_d<FP16, ATTN_CAUSAL>(p, st) : bwd_d<BF16, ATTN_CAUSAL>(p, st);
+  else p.fp16 ? bwd_d<FP16, ATTN_PLAIN>(p, st) : bwd_d<BF16, ATTN_PLAIN>(p, st);
   return hipGetLastError() == hipSuccess ? 0 : 3;
 }

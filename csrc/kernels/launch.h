@@ -637,6 +637,7 @@ struct AttnMask {
 
 struct AttnParams {
   AttnTensor q, k, v, o;            // o: forward output
+  bf16_t* o_rest;                   // o before its rounding less o, laid out like o; kept for the backward (or nullptr)
   AttnTensor go, dq, dk, dv;        // backward
   float* lse2;                      // [B][Hkv][M] log2 of the row's exp2 sum (+inf: empty row); saved for the backward
   float* delta;                     // [B][Hkv][M] workspace of the backward
@@ -645,11 +646,14 @@ struct AttnParams {
   int B, Sq, Sk, Hq, Hkv, G, D, M;  // M = Sq * G
   int causal;
   int fp16;
+  int uneven;                       // blocks differ in work between (image, head)s: attention.h locate()
   float scale;
   FastDiv div_g;
-  int splits;                       // forward: key splits; partial results in ws
-  float* ws_o;                      // [splits][B][Hkv][M][DP]
-  float* ws_ml;                     // [splits][B][Hkv][M][2]
+  int splits;                       // blocks that share the keys of a row block (forward, dq); their parts are in
+  float* ws_o;                      // [splits][B][Hkv][M][DP], DP = D in whole 32s
+  float* ws_ml;                     // [splits][B][Hkv][M][2] (forward)
+  int kv_splits;                    // blocks that share the rows of a key block (dk, dv)
+  float* ws_kv;                     // [2][kv_splits][B][Hkv][Sk][DP]
 };
 
 struct AttnMaskArgs {
@@ -663,6 +667,7 @@ struct AttnMaskArgs {
 int attn_mask_bits(const AttnMaskArgs& a, hipStream_t st);
 int attn_splits(int B, int Hkv, int M, int Sk);      // key splits of a forward call (1: no workspace)
 int attn_fwd(const AttnParams& p, hipStream_t st);
+void attn_bwd_splits(int B, int Hkv, int M, int Sk, int causal, int& splits, int& kv_splits);
 int attn_bwd(const AttnParams& p, hipStream_t st);
 
 // ---------------------------------------------------------------- layer_norm.hip
