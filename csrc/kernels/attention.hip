@@ -209,8 +209,10 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
             for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[k][u][e]);
           mx = fmaxf(mx, other_half(mx)) * sc;
           if (__any(mx > m[u] + SLACK)) {
-            const float mn = fmaxf(m[u], mx), al = exp2_(m[u] - (mn == -INFINITY ? 0.f : mn));
-            m[u] = mn;
+            // only the rows that need it: what a row rounds does not depend on the rows next to it
+            const bool up = mx > m[u] + SLACK;
+            const float al = up ? exp2_(m[u] - mx) : 1.f;
+            m[u] = up ? mx : m[u];
             l[u] *= al;
 #pragma unroll
             for (int d = 0; d < ND; ++d)

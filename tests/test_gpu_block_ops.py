@@ -557,3 +557,198 @@ def test_self_attention2d_gradients_match_64_bits():
     # norm of an error is within about sqrt(12) u of the norm of what it is added to; 6 u leaves the products' gain.
     for n, a, b in zip(["y", "dx", *w], *out):
         assert float((a.double() - b).norm()) <= 6 * half_step(BF) * float(b.norm()), n
+
+
+# ------------------------------------------------------------------------- values that are not finite, where not allowed
+BAD = [math.nan, math.inf, -math.inf]
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("shape", [(2, 90, 130, 4, 2, 64), (2, 1, 300, 2, 2, 32), (1, 150, 200, 2, 1, 128),
+                                   (1, 100, 140, 2, 2, 96)])
+@pytest.mark.parametrize("kind", ["keys", "pairs", "lengths"])
+def test_attention_ignores_what_is_not_allowed(kind, shape, dt):
+    """Keys, values, queries and gradients of tokens that take part in nothing hold NaN and infinities."""
+    B, Sq, Sk, Hq, Hkv, D = shape
+    q, k, v, go = qkvg(*shape, dt)
+    g = torch.Generator().manual_seed(8)
+    dead = torch.rand(Sk, generator=g) < 0.4
+    dead[0] = False
+    kw = {}
+    empty = torch.zeros(Sq, dtype=torch.bool)
+    if kind == "keys":
+        kw["mask"] = (~dead)[None, None, None].expand(B, 1, 1, Sk).contiguous().to(DEV)
+    elif kind == "pairs":
+        m = (torch.rand(Sq, Sk, generator=g) < 0.6) & ~dead
+        if Sq > 3:
+            empty[[1, Sq - 1]] = True
+        m[empty] = False
+        kw["mask"] = m.to(DEV)
+    else:
+        n = Sk - Sk // 3
+        dead = torch.arange(Sk) >= n
+        kw["lengths"] = torch.full((B,), n, dtype=torch.int32, device=DEV)
+    dead, empty = dead.to(DEV), empty.to(DEV)
+    bad = torch.tensor(BAD, dtype=dt, device=DEV)
+    k[:, dead] = bad[torch.arange(int(dead.sum()), device=DEV) % 3][None, :, None, None]
+    v[:, dead] = bad[(torch.arange(int(dead.sum()), device=DEV) + 1) % 3][None, :, None, None]
+    if empty.any():
+        q[:, empty] = math.nan
+        go[:, empty] = math.inf
+    check_attention(q, k, v, go, **kw)
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+def test_attention_causal_ignores_the_future(D, dt):
+    """A value that is not finite shows in the rows that may attend it, in no earlier one; likewise its key."""
+    q, k, v, go = qkvg(1, 150, 150, 2, 2, D, dt)
+    want = ops.attention(q, k, v, causal=True)
+    for t in (v, k):
+        for x in BAD:
+            w = t.clone()
+            w[0, 100, :, 3] = x
+            out = ops.attention(q, w if t is k else k, w if t is v else v, causal=True)
+            ok = allowed(1, 2, 150, 150, causal=True)
+            assert torch.equal(out[:, :100], want[:, :100])
+            if t is v:
+                # the one channel, and there the value itself (a NaN stays one)
+                hit = out[:, 100:, :, 3].float()
+                assert (hit.isnan().all() if math.isnan(x) else (hit == x).all())
+                rest = [c for c in range(D) if c != 3]
+                assert torch.equal(out[..., rest], want[..., rest])
+            else:
+                assert not torch.isfinite(out[:, 100:]).all()
+    # gradients: an infinite gradient of row 40 reaches the keys up to 40 and no later one
+    bad = go.clone()
+    bad[0, 40, :, 5] = math.inf
+    ins = [t.detach().requires_grad_() for t in (q, k, v)]
+    a = torch.autograd.grad(ops.attention(*ins, causal=True), ins, go)
+    b = torch.autograd.grad(ops.attention(*ins, causal=True), ins, bad)
+    for n in (1, 2):
+        assert torch.equal(a[n][:, 41:], b[n][:, 41:])
+    assert (b[2][:, :41, :, 5] == math.inf).all()
+    assert torch.equal(a[2][..., :5], b[2][..., :5])
+    keep = [i for i in range(150) if i != 40]
+    assert torch.equal(a[0][:, keep], b[0][:, keep])
+
+
+def test_attention_masked_rows_hear_nothing_of_a_bad_value():
+    """A dense mask: NaN in one value shows in the rows that attend it only."""
+    q, k, v, _ = qkvg(2, 130, 170, 2, 2, 64, BF)
+    g = torch.Generator().manual_seed(5)
+    mask = torch.rand(130, 170, generator=g) < 0.5
+    mask[:, 0] = True
+    want = ops.attention(q, k, v, mask=mask.to(DEV))
+    v[:, 77] = math.nan
+    out = ops.attention(q, k, v, mask=mask.to(DEV))
+    hit = mask[:, 77].to(DEV)
+    assert out[:, hit].isnan().all()
+    assert torch.equal(out[:, ~hit], want[:, ~hit])
+
+
+def test_attention_infinite_gradient_is_not_lost():
+    """Overflow of a scaled loss: an infinite gradient must reach every gradient that depends on it."""
+    q, k, v, go = qkvg(1, 70, 90, 2, 2, 64, HF)
+    go[0, 30, 1] = math.inf
+    for kw in ({}, {"causal": True}, {"mask": torch.ones(70, 90, dtype=torch.bool, device=DEV)}):
+        ins = [t.detach().requires_grad_() for t in (q, k, v)]
+        dq, dk, dv = torch.autograd.grad(ops.attention(*ins, **kw), ins, go)
+        assert not torch.isfinite(dq[0, 30, 1]).any()
+        assert not torch.isfinite(dv[0, :40, 1]).any()
+        assert not torch.isfinite(dk[0, :40, 1]).any()
+        assert torch.isfinite(dv[0, :, 0]).all() and torch.isfinite(dk[0, :, 0]).all()
+
+
+# --------------------------------------------------------------------------------------------- streams, graphs, reuse
+def test_ops_run_on_the_current_stream():
+    x, w = rnd((4096, 256), BF, 0), rnd((256,), FF, 1)
+    q, k, v, go = qkvg(2, 300, 300, 4, 4, 64, BF)
+    pos = ops.grid_positions(15, 20, device=DEV)
+    mask = (torch.rand(300, 300, generator=torch.Generator().manual_seed(1)) < 0.5).to(DEV)
+
+    def run():
+        ins = [t.detach().requires_grad_() for t in (q, k, v, x, w)]
+        a = ops.attention(ops.rotary(ins[0], pos, (32, 32)), ops.rotary(ins[1], pos, (32, 32)), ins[2], mask)
+        b = ops.layer_norm(ins[3], ins[4])
+        return [a.detach(), b.detach(), *torch.autograd.grad([a, b], ins, [go, x])]
+
+    want = run()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = run()
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_two_captured_graphs_replay_in_any_order():
+    """Forward and backward captured twice, with splits, masks and the weights' gradient sums: each graph keeps its own
+    workspaces, replays follow its inputs, and eager work between the replays changes nothing."""
+    def case(seed, Sq, Sk):
+        q, k, v, go = qkvg(1, Sq, Sk, 2, 2, 64, BF, seed)
+        x, w, gy = rnd((500, 96), BF, seed), rnd((96,), FF, seed + 1), rnd((500, 96), BF, seed + 2)
+        mask = (torch.rand(Sk, generator=torch.Generator().manual_seed(seed)) < 0.8)[None, None, None].to(DEV)
+        pos = torch.arange(Sq, device=DEV, dtype=torch.int32)[None]
+        leaves = [t.requires_grad_() for t in (q, k, v, x, w)]
+
+        def run():
+            a = ops.attention(ops.rotary(leaves[0], pos, (64,)), leaves[1], leaves[2], mask)
+            b = ops.layer_norm(leaves[3], leaves[4])
+            return [a.detach(), b.detach(), *torch.autograd.grad([a, b], leaves, [go, gy])]
+        return leaves, run
+
+    made = []
+    for seed, Sq, Sk in ((1, 20, 2000), (50, 700, 150)):
+        leaves, run = case(seed, Sq, Sk)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+        made.append((leaves, run, graph, out))
+    for step in range(3):
+        for leaves, run, graph, out in made if step % 2 else made[::-1]:
+            with torch.no_grad():
+                for t in leaves:
+                    t.mul_(0.9)
+            graph.replay()
+            torch.cuda.synchronize()
+            got = [t.clone() for t in out]
+            for a, b in zip(got, run()):
+                assert torch.equal(a, b)
+
+
+def test_attention_long_keys_and_far_offsets():
+    """One query over 300,000 keys whose rows span more than 2^31 bytes; the last keys count."""
+    S, wide = 300_000, 4096
+    kv = torch.zeros(1, S, 1, wide, dtype=BF, device=DEV)
+    kv[..., :16] = rnd((1, S, 1, 16), BF, 0)
+    kv[..., 16:32] = rnd((1, S, 1, 16), BF, 1)
+    k, v = kv[..., :16], kv[..., 16:32]
+    assert S * wide * 2 > 2 ** 31
+    q = rnd((1, 1, 1, 16), BF, 2)
+    check_attention(q, k, v, rnd((1, 1, 1, 16), BF, 3))
+    k[0, S - 1] = 8 * q[0, 0]
+    v[0, S - 1] = 5.0
+    out = ops.attention(q, k, v, scale=2.0)
+    assert (out == 5.0).all()
+
+
+def test_attention_mask_past_the_table_of_tiles():
+    """Keys beyond the tiles whose class a block keeps: processed, masked all the same."""
+    S = 64 * 2048 + 500
+    q, k, v, go = qkvg(1, 3, S, 1, 1, 8, BF)
+    mask = (torch.rand(1, 1, 1, S, generator=torch.Generator().manual_seed(2)) < 0.5).to(DEV)
+    mask[..., 64 * 2048 + 128:64 * 2048 + 300] = False
+    check_attention(q, k, v, go, mask=mask)
+    many = 32 * 2048 + 200                                   # as many rows, walked by the keys' blocks
+    q, k, v, go = qkvg(1, many, 40, 1, 1, 8, BF)
+    mask = (torch.rand(many, 40, generator=torch.Generator().manual_seed(3)) < 0.5).to(DEV)
+    check_attention(q, k, v, go, mask=mask)
