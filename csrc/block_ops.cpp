@@ -483,9 +483,9 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     p.y = nx ? r[0].data_ptr() : nullptr;
     p.dw = nw ? r[1].data_ptr<float>() : nullptr;
     p.db = nb ? r[2].data_ptr<float>() : nullptr;
-    p.blocks = layer_norm_bwd_blocks(p.rows, p.C);
+    p.blocks = layer_norm_bwd_blocks(p);
     at::Tensor ws;
-    if (nw || nb) {
+    if ((nw || nb) && p.blocks > 1) {
       ws = at::empty({(int64_t)p.blocks * 2 * C}, f32);
       p.ws = ws.data_ptr<float>();
     }

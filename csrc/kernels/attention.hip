@@ -377,7 +377,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnParams p) {
   if (d == 0 && p.lse2) p.lse2[row] = l == 0.f ? INFINITY : mn + __builtin_amdgcn_logf(l);
 }
 
-// mask bytes -> words: one wave per (32 mask rows, 64 keys)
+// mask bytes -> words: one wave per (32 mask rows, 64 keys), all of its loads under way together
 __global__ __launch_bounds__(256) void attn_mask_kernel(const AttnMaskArgs a) {
   const int nib = (a.Im + 31) >> 5, lane = threadIdx.x & 63;
   const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), per = (int64_t)nib * a.words;
@@ -386,16 +386,19 @@ __global__ __launch_bounds__(256) void attn_mask_kernel(const AttnMaskArgs a) {
   const int ib = (int)((unit - lead * per) / a.words), w = (int)(unit % a.words);
   const int b = (int)(lead / a.Hm), h = (int)(lead % a.Hm), key = 64 * w + lane;
   const uint8_t* src = a.src + b * a.sb + h * a.sh + (int64_t)imin(key, a.Sk - 1) * a.sk;
-  unsigned long long any = 0, all = ~0ull;
   const int n = imin(32, a.Im - 32 * ib);
-#pragma unroll 8
-  for (int k = 0; k < n; ++k) {
-    const int i = 32 * ib + k;
-    const unsigned long long bits = __ballot(key < a.Sk && src[(int64_t)i * a.si] != 0);
+  uint8_t v[32];
+#pragma unroll
+  for (int k = 0; k < 32; ++k) v[k] = src[(int64_t)(32 * ib + imin(k, n - 1)) * a.si];
+  unsigned long long any = 0, all = ~0ull, mine = 0;
+#pragma unroll
+  for (int k = 0; k < 32; ++k) {
+    const unsigned long long bits = __ballot(key < a.Sk && v[k] != 0);   // rows past the last repeat it
     any |= bits;
     all &= bits;
-    if (lane == 0) a.bits[(lead * a.Im + i) * a.words + w] = bits;
+    mine = lane == k ? bits : mine;
   }
+  if (lane < n) a.bits[(lead * a.Im + 32 * ib + lane) * a.words + w] = mine;
   if (lane == 0) a.cls[unit] = any == 0 ? 0 : all == ~0ull ? 2 : 1;
 }
 

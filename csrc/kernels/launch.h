@@ -671,7 +671,7 @@ void attn_bwd_splits(int B, int Hkv, int M, int Sk, int causal, int& splits, int
 int attn_bwd(const AttnParams& p, hipStream_t st);
 
 // ---------------------------------------------------------------- layer_norm.hip
-constexpr int LAYER_NORM_MAX_C = 16384;       // a row is held in registers: 1,024 lanes of 16
+constexpr int LAYER_NORM_MAX_C = 8192;        // a row is held in registers: 512 lanes of 16
 struct LayerNormParams {
   const void* x;           // [rows][C], row stride x_stride
   const void* gy;          // backward
@@ -688,7 +688,7 @@ struct LayerNormParams {
   int blocks;
 };
 int layer_norm_fwd(const LayerNormParams& p, hipStream_t st);
-int layer_norm_bwd_blocks(int64_t rows, int C);
+int layer_norm_bwd_blocks(const LayerNormParams& p);
 int layer_norm_bwd(const LayerNormParams& p, hipStream_t st);
 
 // ---------------------------------------------------------------- rotary.hip

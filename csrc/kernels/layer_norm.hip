@@ -39,282 +39,356 @@ struct Elem<2> {
   static CFL_DEVICE _Float16 put(float v) { return (_Float16)v; }
 };
 
-// V consecutive elements as floats (V = 1, or a 16-byte vector)
+// V consecutive elements (V = 1, or a 16-byte vector), as they lie in memory
 template <int TYPE, int V>
-CFL_DEVICE void load_v(const typename Elem<TYPE>::type* p, float* f) {
-  typedef typename Elem<TYPE>::type E;
-  if constexpr (V == 1) {
-    f[0] = Elem<TYPE>::get(*p);
-  } else {
-    struct alignas(16) Vec { E e[V]; };
-    const Vec v = *reinterpret_cast<const Vec*>(p);
+struct alignas(V * sizeof(typename Elem<TYPE>::type)) Vec {
+  typename Elem<TYPE>::type e[V];
+};
+
+// the vectors of this lane's columns of a row; columns past C read as 0
+template <int TYPE, int V, int NV>
+CFL_DEVICE void load_row(const typename Elem<TYPE>::type* row, const int* col, int C, bool ok, Vec<TYPE, V>* v) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = Elem<TYPE>::get(v.e[j]);
+  for (int k = 0; k < NV; ++k) {
+    Vec<TYPE, V> t = {};
+    if (ok && col[k] < C) t = *reinterpret_cast<const Vec<TYPE, V>*>(row + col[k]);
+    v[k] = t;
   }
 }
 template <int TYPE, int V>
 CFL_DEVICE void store_v(typename Elem<TYPE>::type* p, const float* f) {
-  typedef typename Elem<TYPE>::type E;
-  if constexpr (V == 1) {
-    *p = Elem<TYPE>::put(f[0]);
-  } else {
-    struct alignas(16) Vec { E e[V]; };
-    Vec v;
+  Vec<TYPE, V> v;
 #pragma unroll
-    for (int j = 0; j < V; ++j) v.e[j] = Elem<TYPE>::put(f[j]);
-    *reinterpret_cast<Vec*>(p) = v;
-  }
+  for (int j = 0; j < V; ++j) v.e[j] = Elem<TYPE>::put(f[j]);
+  *reinterpret_cast<Vec<TYPE, V>*>(p) = v;
 }
 
-// NSUM sums over the LPR lanes of a row, the result in each of them. Groups inside a wave exchange lanes; a block-wide
-// row (LPR > 64) goes through LDS: `red` holds NSUM * LPR / 64 floats, one barrier pair per call.
-template <int LPR, int NSUM>
-CFL_DEVICE void row_sum(float* v, float* red) {
+// a sum over the row's lanes of one wave (all of them where LPR <= 64)
+template <int LPR>
+CFL_DEVICE float lane_sum(float v) {
 #pragma unroll
-  for (int n = 0; n < NSUM; ++n)
-#pragma unroll
-    for (int o = 1; o < (LPR < 64 ? LPR : 64); o <<= 1) v[n] = xor_add(v[n], o);
-  if constexpr (LPR > 64) {
-    constexpr int W = LPR / 64;
-    if ((threadIdx.x & 63) == 0)
-#pragma unroll
-      for (int n = 0; n < NSUM; ++n) red[n * W + (threadIdx.x >> 6)] = v[n];
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < NSUM; ++n) {
-      float t = 0.f;
-#pragma unroll
-      for (int w = 0; w < W; ++w) t += red[n * W + w];
-      v[n] = t;
-    }
-    __syncthreads();
-  }
+  for (int o = 1; o < (LPR < 64 ? LPR : 64); o <<= 1) v = xor_add(v, o);
+  return v;
 }
 
-// mu and r of the row held in x; masked elements (columns past C) hold 0 on entry and on return x - mu is 0 there
+// What the statistics need that is the same for every row: 1 / C and, for a row of several waves, the columns of this
+// wave and of each.
+template <int LPR>
+struct RowShape {
+  static constexpr int W = LPR > 64 ? LPR / 64 : 1;
+  float inv, own;                // 1 / C; 1 / columns of this wave (0: none)
+  float part[W];                 // columns of each wave
+};
 template <int LPR, int NV, int V>
-CFL_DEVICE float center(float (*x)[V], const int* col, int C, float eps, float* red) {
+CFL_DEVICE RowShape<LPR> row_shape(int C) {
+  RowShape<LPR> s;
+  s.inv = 1.f / (float)C;
+  s.own = s.inv;
+  if constexpr (LPR > 64) {
+#pragma unroll
+    for (int u = 0; u < LPR / 64; ++u) {
+      int n = 0;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) n += imax(0, imin(C - (k * LPR + 64 * u) * V, 64 * V));
+      s.part[u] = (float)n;
+      if (u == (int)(threadIdx.x % LPR) >> 6) s.own = n > 0 ? 1.f / (float)n : 0.f;
+    }
+  }
+  return s;
+}
+
+// x -> x less the mean of this wave's columns (0 in the columns past C); returns r, and in `d` what has to be added to
+// the columns of vector k for x - mu. A row of several waves joins the waves' own means and sums of squares:
+// M2 = sum M2_w + n_w (mu_w - mu)^2, with one exchange through LDS. `red` alternates between two buffers from row to row,
+// so one barrier per exchange is enough: a buffer is written again only after a barrier that every wave reaches behind
+// its reads.
+template <int LPR, int NV, int V>
+CFL_DEVICE float center(float (*x)[V], const int* col, int C, float eps, const RowShape<LPR>& sh, float2* red,
+                        float* d) {
   float s = 0.f;
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
     for (int j = 0; j < V; ++j) s += x[k][j];
-  row_sum<LPR, 1>(&s, red);
-  const float mu = s / (float)C;
+  const float mw = lane_sum<LPR>(s) * sh.own;
   float q = 0.f;
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
+  for (int k = 0; k < NV; ++k) {
+    const float mk = col[k] < C ? mw : 0.f;                // the columns past C hold 0 and stay 0
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      x[k][j] = col[k] < C ? x[k][j] - mu : 0.f;
+      x[k][j] -= mk;
       q = fmaf(x[k][j], x[k][j], q);
     }
-  row_sum<LPR, 1>(&q, red);
-  return 1.f / sqrtf(q / (float)C + eps);
+    d[k] = 0.f;
+  }
+  q = lane_sum<LPR>(q);
+  if constexpr (LPR > 64) {
+    constexpr int W = LPR / 64;
+    if ((threadIdx.x & 63) == 0) red[(threadIdx.x % LPR) >> 6] = make_float2(mw, q);
+    __syncthreads();
+    float2 w[W];
+    float mu = 0.f;
+#pragma unroll
+    for (int u = 0; u < W; ++u) {
+      w[u] = red[u];
+      mu = fmaf(w[u].x, sh.part[u], mu);
+    }
+    mu *= sh.inv;
+    q = 0.f;
+#pragma unroll
+    for (int u = 0; u < W; ++u) q += fmaf(sh.part[u] * (w[u].x - mu), w[u].x - mu, w[u].y);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) d[k] = col[k] < C ? mw - mu : 0.f;
+  }
+  return rsqrtf(fmaf(q, sh.inv, eps));
 }
 
-template <int LPR>
-constexpr int threads() { return LPR > 256 ? LPR : 256; }
+// a lane's columns of a fp32 weight (`dflt` where there is none, or past C)
+template <int NV, int V>
+CFL_DEVICE void load_weight(const float* p, const int* col, int C, float dflt, float (*w)[V]) {
+  const bool vec = V >= 4 && p != nullptr && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) w[k][j] = dflt;
+    if (p == nullptr || col[k] >= C) continue;
+    if (vec) {
+#pragma unroll
+      for (int j = 0; j + 3 < V; j += 4) {
+        const float4 t = *reinterpret_cast<const float4*>(p + col[k] + j);
+        w[k][j] = t.x; w[k][j + 1] = t.y; w[k][j + 2] = t.z; w[k][j + 3] = t.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) w[k][j] = p[col[k] + j];
+    }
+  }
+}
 
 // rows go to row groups (LPR lanes) in turn; NV vectors of V elements a lane: vector k of lane q starts at column
-// (k LPR + q) V
-template <int TYPE, int V, int LPR, int NV>
-__global__ __launch_bounds__(threads<LPR>()) void ln_fwd_kernel(const LayerNormParams p) {
+// (k LPR + q) V. The next row's loads are under way while a row is worked on.
+template <int TYPE, int V, int LPR, int NV, int NT>
+__global__ __launch_bounds__(NT) void ln_fwd_kernel(const LayerNormParams p) {
   typedef typename Elem<TYPE>::type E;
-  constexpr int NT = threads<LPR>(), RPB = NT / LPR;
-  __shared__ float red[LPR > 64 ? LPR / 64 : 1];
-  const int q = threadIdx.x % LPR;
+  constexpr int RPB = NT / LPR;
+  __shared__ float2 red[2][RPB][LPR > 64 ? LPR / 64 : 1];
+  const int q = threadIdx.x % LPR, g = threadIdx.x / LPR;
   int col[NV];
   float w[NV][V], b[NV][V];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     col[k] = (k * LPR + q) * V;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const bool in = col[k] < p.C;
-      w[k][j] = in && p.w ? p.w[col[k] + j] : 1.f;
-      b[k][j] = in && p.b ? p.b[col[k] + j] : 0.f;
-    }
   }
-  for (int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR; r - threadIdx.x / LPR < p.rows;
-       r += (int64_t)gridDim.x * RPB) {
+  load_weight<NV, V>(p.w, col, p.C, 1.f, w);
+  load_weight<NV, V>(p.b, col, p.C, 0.f, b);
+  const RowShape<LPR> sh = row_shape<LPR, NV, V>(p.C);
+  const E* xb = reinterpret_cast<const E*>(p.x);
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t r = (int64_t)blockIdx.x * RPB + g;
+  Vec<TYPE, V> xn[NV];
+  load_row<TYPE, V, NV>(xb + r * p.x_stride, col, p.C, r < p.rows, xn);
+  for (int par = 0; r - g < p.rows; r += step, par ^= 1) {
     const bool ok = r < p.rows;
-    const E* xr = reinterpret_cast<const E*>(p.x) + r * p.x_stride;
     float x[NV][V];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
+    for (int k = 0; k < NV; ++k)
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[k][j] = 0.f;
-      if (ok && col[k] < p.C) load_v<TYPE, V>(xr + col[k], x[k]);
-    }
-    const float rs = center<LPR, NV, V>(x, col, p.C, p.eps, red);
+      for (int j = 0; j < V; ++j) x[k][j] = Elem<TYPE>::get(xn[k].e[j]);
+    load_row<TYPE, V, NV>(xb + (r + step) * p.x_stride, col, p.C, r + step < p.rows, xn);
+    float d[NV];
+    const float rs = center<LPR, NV, V>(x, col, p.C, p.eps, sh, red[par][g], d);
     E* yr = reinterpret_cast<E*>(p.y) + r * p.C;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[k][j] = fmaf(x[k][j] * rs, w[k][j], b[k][j]);
+      for (int j = 0; j < V; ++j) x[k][j] = fmaf(fmaf(x[k][j], rs, d[k] * rs), w[k][j], b[k][j]);
       if (ok && col[k] < p.C) store_v<TYPE, V>(yr + col[k], x[k]);
     }
   }
 }
 
-template <int TYPE, int V, int LPR, int NV>
-__global__ __launch_bounds__(threads<LPR>()) void ln_bwd_kernel(const LayerNormParams p) {
+template <int TYPE, int V, int LPR, int NV, int NT>
+__global__ __launch_bounds__(NT) void ln_bwd_kernel(const LayerNormParams p) {
   typedef typename Elem<TYPE>::type E;
-  constexpr int NT = threads<LPR>(), RPB = NT / LPR;
-  __shared__ float red[LPR > 64 ? 2 * (LPR / 64) : 1];
-  const int q = threadIdx.x % LPR;
+  constexpr int RPB = NT / LPR;
+  __shared__ float2 red[2][RPB][LPR > 64 ? LPR / 64 : 1], red2[2][RPB][LPR > 64 ? LPR / 64 : 1];
+  const int q = threadIdx.x % LPR, gr = threadIdx.x / LPR;
   int col[NV];
   float w[NV][V], dw[NV][V], db[NV][V];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     col[k] = (k * LPR + q) * V;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      w[k][j] = col[k] < p.C && p.w ? p.w[col[k] + j] : 1.f;
-      dw[k][j] = db[k][j] = 0.f;
-    }
+    for (int j = 0; j < V; ++j) dw[k][j] = db[k][j] = 0.f;
   }
-  for (int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR; r - threadIdx.x / LPR < p.rows;
-       r += (int64_t)gridDim.x * RPB) {
+  load_weight<NV, V>(p.w, col, p.C, 1.f, w);
+  const RowShape<LPR> sh = row_shape<LPR, NV, V>(p.C);
+  const E *xb = reinterpret_cast<const E*>(p.x), *gb = reinterpret_cast<const E*>(p.gy);
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t r = (int64_t)blockIdx.x * RPB + gr;
+  Vec<TYPE, V> xn[NV], gn[NV];
+  load_row<TYPE, V, NV>(xb + r * p.x_stride, col, p.C, r < p.rows, xn);
+  load_row<TYPE, V, NV>(gb + r * p.gy_stride, col, p.C, r < p.rows, gn);
+  for (int par = 0; r - gr < p.rows; r += step, par ^= 1) {
     const bool ok = r < p.rows;
-    const E* xr = reinterpret_cast<const E*>(p.x) + r * p.x_stride;
-    const E* gr = reinterpret_cast<const E*>(p.gy) + r * p.gy_stride;
     float x[NV][V], g[NV][V];
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) x[k][j] = g[k][j] = 0.f;
-      if (ok && col[k] < p.C) {
-        load_v<TYPE, V>(xr + col[k], x[k]);
-        load_v<TYPE, V>(gr + col[k], g[k]);
-      }
-    }
-    const float rs = center<LPR, NV, V>(x, col, p.C, p.eps, red);
-    float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        x[k][j] *= rs;
+        x[k][j] = Elem<TYPE>::get(xn[k].e[j]);
+        g[k][j] = Elem<TYPE>::get(gn[k].e[j]);
+      }
+    load_row<TYPE, V, NV>(xb + (r + step) * p.x_stride, col, p.C, r + step < p.rows, xn);
+    load_row<TYPE, V, NV>(gb + (r + step) * p.gy_stride, col, p.C, r + step < p.rows, gn);
+    float d[NV];
+    const float rs = center<LPR, NV, V>(x, col, p.C, p.eps, sh, red[par][gr], d);
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        x[k][j] = fmaf(x[k][j], rs, d[k] * rs);
         dw[k][j] = fmaf(g[k][j], x[k][j], dw[k][j]);
         db[k][j] += g[k][j];
         g[k][j] *= w[k][j];
-        s[0] += g[k][j];
-        s[1] = fmaf(g[k][j], x[k][j], s[1]);
+        s0 += g[k][j];
+        s1 = fmaf(g[k][j], x[k][j], s1);
       }
     if (p.y == nullptr) continue;
-    row_sum<LPR, 2>(s, red);
-    const float m0 = s[0] / (float)p.C, m1 = s[1] / (float)p.C;
+    s0 = lane_sum<LPR>(s0);
+    s1 = lane_sum<LPR>(s1);
+    if constexpr (LPR > 64) {
+      if ((threadIdx.x & 63) == 0) red2[par][gr][q >> 6] = make_float2(s0, s1);
+      __syncthreads();
+      s0 = s1 = 0.f;
+#pragma unroll
+      for (int u = 0; u < LPR / 64; ++u) {
+        s0 += red2[par][gr][u].x;
+        s1 += red2[par][gr][u].y;
+      }
+    }
+    const float m0 = -s0 * sh.inv * rs, m1 = -s1 * sh.inv * rs;
     E* yr = reinterpret_cast<E*>(p.y) + r * p.C;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[k][j] = rs * (g[k][j] - m0 - x[k][j] * m1);
+      for (int j = 0; j < V; ++j) x[k][j] = fmaf(x[k][j], m1, fmaf(g[k][j], rs, m0));
       if (ok && col[k] < p.C) store_v<TYPE, V>(yr + col[k], x[k]);
     }
   }
-  if (p.ws == nullptr) return;
-  // join the row groups that own the same columns, one vector at a time: lanes of a wave, then the block's waves
-  constexpr int W = RPB > 1 ? (LPR < 64 ? NT / 64 : RPB) : 1, G = LPR < 64 ? LPR : 64;
-  __shared__ float part[W > 1 ? W * G * 2 * V : 1];
-  float* out = p.ws + (int64_t)blockIdx.x * 2 * p.C;
+  if (p.dw == nullptr && p.db == nullptr) return;
+  // join the row groups that own the same columns: lanes of a wave, then the block's waves, one element of every lane at
+  // a time through LDS. J waves hold a wave-wide set of columns each.
+  constexpr int J = LPR > 64 ? RPB : NT / 64, G = LPR < 64 ? LPR : 64;
+  __shared__ float2 part[J > 1 ? NT / 64 * G : 1];
+  // one block: its sums are the result
+  float* odw = gridDim.x == 1 ? p.dw : p.ws + (int64_t)blockIdx.x * 2 * p.C;
+  float* odb = gridDim.x == 1 ? p.db : p.ws + (int64_t)blockIdx.x * 2 * p.C + p.C;
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
+  for (int k = 0; k < NV; ++k)
 #pragma unroll
-    for (int j = 0; j < V; ++j)
+    for (int j = 0; j < V; ++j) {
+      float2 t = make_float2(dw[k][j], db[k][j]);
 #pragma unroll
       for (int o = G; o < 64; o <<= 1) {
-        dw[k][j] = xor_add(dw[k][j], o);
-        db[k][j] = xor_add(db[k][j], o);
+        t.x = xor_add(t.x, o);
+        t.y = xor_add(t.y, o);
       }
-    if constexpr (W > 1) {
-      const int wv = threadIdx.x >> 6, l = threadIdx.x & 63;
-      if (k > 0) __syncthreads();
-      if (l < G)
+      if constexpr (J > 1) {
+        constexpr int SETS = LPR > 64 ? LPR / 64 : 1;      // waves of one row
+        const int wv = threadIdx.x >> 6, l = threadIdx.x & 63;
+        if (k + j > 0) __syncthreads();
+        if (l < G) part[wv * G + l] = t;
+        __syncthreads();
+        if (wv < SETS && l < G) {
+          t = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          part[((wv * 2) * V + j) * G + l] = dw[k][j];
-          part[((wv * 2 + 1) * V + j) * G + l] = db[k][j];
-        }
-      __syncthreads();
-      if (threadIdx.x < G)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          float a = 0.f, b = 0.f;
-#pragma unroll
-          for (int u = 0; u < W; ++u) {
-            a += part[((u * 2) * V + j) * G + l];
-            b += part[((u * 2 + 1) * V + j) * G + l];
+          for (int u = 0; u < J; ++u) {
+            const float2 v = part[(u * SETS + wv) * G + l];
+            t.x += v.x;
+            t.y += v.y;
           }
-          dw[k][j] = a;
-          db[k][j] = b;
         }
-    }
-    if (threadIdx.x < LPR && col[k] < p.C)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        out[col[k] + j] = dw[k][j];
-        out[p.C + col[k] + j] = db[k][j];
       }
-  }
+      if (threadIdx.x < LPR && col[k] < p.C) {
+        if (odw) odw[col[k] + j] = t.x;
+        if (odb) odb[col[k] + j] = t.y;
+      }
+    }
 }
 
-// dw / db = sums of the partial rows: a block owns 32 columns of one of the two, 8 threads a column
-__global__ __launch_bounds__(256) void ln_bwd_join_kernel(const LayerNormParams p) {
-  __shared__ float s[8][33];
+// dw / db = sums of the partial rows: a block owns 32 columns of one of the two, 32 threads a column
+__global__ __launch_bounds__(1024) void ln_bwd_join_kernel(const LayerNormParams p) {
+  __shared__ float s[32][33];
   const int cl = threadIdx.x & 31, g = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
   float* out = blockIdx.y ? p.db : p.dw;
   if (out == nullptr) return;
   float a = 0.f;
   if (c < p.C) {
     const float* src = p.ws + (int64_t)blockIdx.y * p.C + c;
-#pragma unroll 4
-    for (int b = g; b < p.blocks; b += 8) a += src[(int64_t)b * 2 * p.C];
+#pragma unroll 8
+    for (int b = g; b < p.blocks; b += 32) a += src[(int64_t)b * 2 * p.C];
   }
   s[g][cl] = a;
   __syncthreads();
   if (g == 0 && c < p.C) {
     float t = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) t += s[k][cl];
+    for (int k = 0; k < 32; ++k) t += s[k][cl];
     out[c] = t;
   }
 }
 
+// Backward: 512 threads (256 registers each: 16 elements of x, dy, w, dw, db and the next row's vectors) and up to 512
+// blocks. Fewer blocks leave memory idle, more cost partial rows of dw and db: 16,384 x 4,096 fp16 121 / 106 / 111 us
+// and 32,768 x 1,024 bf16 48 / 41 / 45 us for 256 / 512 / 1,024 blocks; 1,024 threads 114 and 48 us for 512 blocks.
+// Forward: 256 threads; more than 2,048 blocks load w and b too often (32,768 x 1,024: 65 us for 8,192, 22 for 2,048).
+constexpr int bwd_threads = 512;
+
 template <int TYPE, int V, int LPR, int NV>
-void go(const LayerNormParams& p, bool bwd, hipStream_t st) {
-  constexpr int NT = threads<LPR>(), RPB = NT / LPR;
-  if (bwd) {
-    ln_bwd_kernel<TYPE, V, LPR, NV><<<p.blocks, NT, 0, st>>>(p);
-  } else {
-    const int64_t n = (p.rows + RPB - 1) / RPB;
-    ln_fwd_kernel<TYPE, V, LPR, NV><<<(unsigned)std::min<int64_t>(n, 4096), NT, 0, st>>>(p);
-  }
+int go(const LayerNormParams& p, bool bwd, bool count, hipStream_t st) {
+  constexpr int NT = bwd_threads, RPB = NT / LPR, NTF = LPR > 256 ? LPR : 256, RPBF = NTF / LPR;
+  static_assert(LPR <= NT, "a row fits the block");
+  if (count) return (int)std::min<int64_t>(512, (p.rows + RPB - 1) / RPB);
+  if (bwd)
+    ln_bwd_kernel<TYPE, V, LPR, NV, NT><<<p.blocks, NT, 0, st>>>(p);
+  else
+    ln_fwd_kernel<TYPE, V, LPR, NV, NTF>
+        <<<(unsigned)std::min<int64_t>(2048, (p.rows + RPBF - 1) / RPBF), NTF, 0, st>>>(p);
+  return hipGetLastError() == hipSuccess ? 0 : 3;
 }
 
 // lanes per row by the row's vectors: the smallest group that holds it
 template <int TYPE, int V>
-int pick(const LayerNormParams& p, bool bwd, hipStream_t st) {
+int pick(const LayerNormParams& p, bool bwd, bool count, hipStream_t st) {
   const int n = (p.C + V - 1) / V;
-  if (n <= 4) go<TYPE, V, 4, 1>(p, bwd, st);
-  else if (n <= 8) go<TYPE, V, 8, 1>(p, bwd, st);
-  else if (n <= 16) go<TYPE, V, 16, 1>(p, bwd, st);
-  else if (n <= 32) go<TYPE, V, 32, 1>(p, bwd, st);
-  else if (n <= 64) go<TYPE, V, 64, 1>(p, bwd, st);
-  else if (n <= 128) go<TYPE, V, 64, 2>(p, bwd, st);
-  else if (n <= 256) go<TYPE, V, 64, 4>(p, bwd, st);
-  else if constexpr (V == 1) {
-    if (n <= 512) go<TYPE, V, 64, 8>(p, bwd, st);
-    else if (n <= 2048) go<TYPE, V, 256, 8>(p, bwd, st);
-    else if (n <= 8192) go<TYPE, V, 1024, 8>(p, bwd, st);
-    else go<TYPE, V, 1024, 16>(p, bwd, st);
+  if (n <= 4) return go<TYPE, V, 4, 1>(p, bwd, count, st);
+  if (n <= 8) return go<TYPE, V, 8, 1>(p, bwd, count, st);
+  if (n <= 16) return go<TYPE, V, 16, 1>(p, bwd, count, st);
+  if (n <= 32) return go<TYPE, V, 32, 1>(p, bwd, count, st);
+  if (n <= 64) return go<TYPE, V, 64, 1>(p, bwd, count, st);
+  if constexpr (V == 8) {
+    if (n <= 128) return go<TYPE, V, 128, 1>(p, bwd, count, st);
+    if (n <= 256) return go<TYPE, V, 256, 1>(p, bwd, count, st);
+    if (n <= 512) return go<TYPE, V, 512, 1>(p, bwd, count, st);
+    return go<TYPE, V, 512, 2>(p, bwd, count, st);
+  } else if constexpr (V == 4) {
+    if (n <= 128) return go<TYPE, V, 64, 2>(p, bwd, count, st);
+    if (n <= 256) return go<TYPE, V, 128, 2>(p, bwd, count, st);
+    if (n <= 512) return go<TYPE, V, 256, 2>(p, bwd, count, st);
+    if (n <= 1024) return go<TYPE, V, 512, 2>(p, bwd, count, st);
+    return go<TYPE, V, 512, 4>(p, bwd, count, st);
   } else {
-    if (n <= 512) go<TYPE, V, 256, 2>(p, bwd, st);
-    else if (n <= 1024) go<TYPE, V, 256, 4>(p, bwd, st);
-    else go<TYPE, V, 1024, 16 / V>(p, bwd, st);
+    if (n <= 128) return go<TYPE, V, 64, 2>(p, bwd, count, st);
+    if (n <= 256) return go<TYPE, V, 64, 4>(p, bwd, count, st);
+    if (n <= 512) return go<TYPE, V, 64, 8>(p, bwd, count, st);
+    if (n <= 1024) return go<TYPE, V, 128, 8>(p, bwd, count, st);
+    if (n <= 2048) return go<TYPE, V, 256, 8>(p, bwd, count, st);
+    if (n <= 4096) return go<TYPE, V, 512, 8>(p, bwd, count, st);
+    return go<TYPE, V, 512, 16>(p, bwd, count, st);
   }
-  return hipGetLastError() == hipSuccess ? 0 : 3;
 }
 
 bool aligned(const void* p, int64_t stride, int C, int V, int size) {
@@ -322,35 +396,35 @@ bool aligned(const void* p, int64_t stride, int C, int V, int size) {
 }
 
 template <int TYPE>
-int run(const LayerNormParams& p, bool bwd, hipStream_t st) {
+int run(const LayerNormParams& p, bool bwd, bool count, hipStream_t st) {
   constexpr int V = Elem<TYPE>::V, size = sizeof(typename Elem<TYPE>::type);
   const bool vec = aligned(p.x, p.x_stride, p.C, V, size) && (!bwd || aligned(p.gy, p.gy_stride, p.C, V, size));
-  return vec ? pick<TYPE, V>(p, bwd, st) : pick<TYPE, 1>(p, bwd, st);
+  return vec ? pick<TYPE, V>(p, bwd, count, st) : pick<TYPE, 1>(p, bwd, count, st);
 }
 
-int run_type(const LayerNormParams& p, bool bwd, hipStream_t st) {
-  if (p.C < 1 || p.rows < 1 || p.C > LAYER_NORM_MAX_C) return 1;
+int run_type(const LayerNormParams& p, bool bwd, bool count, hipStream_t st) {
   switch (p.type) {
-    case 0: return run<0>(p, bwd, st);
-    case 1: return run<1>(p, bwd, st);
-    case 2: return run<2>(p, bwd, st);
-    default: return 1;
+    case 0: return run<0>(p, bwd, count, st);
+    case 1: return run<1>(p, bwd, count, st);
+    default: return run<2>(p, bwd, count, st);
   }
+}
+
+bool valid(const LayerNormParams& p) {
+  return p.C >= 1 && p.C <= LAYER_NORM_MAX_C && p.rows >= 1 && p.type >= 0 && p.type <= 2;
 }
 
 }  // namespace
 
-int layer_norm_fwd(const LayerNormParams& p, hipStream_t st) { return run_type(p, false, st); }
+int layer_norm_fwd(const LayerNormParams& p, hipStream_t st) { return valid(p) ? run_type(p, false, false, st) : 1; }
 
 // blocks of the backward pass = partial rows of dw / db
-int layer_norm_bwd_blocks(int64_t rows, int C) {
-  const int64_t per = C <= 64 ? 32 : 4;            // rows a block holds at a time, at least
-  return (int)std::max<int64_t>(1, std::min<int64_t>(512, (rows + per - 1) / per));
-}
+int layer_norm_bwd_blocks(const LayerNormParams& p) { return valid(p) ? run_type(p, true, true, nullptr) : 0; }
 
 int layer_norm_bwd(const LayerNormParams& p, hipStream_t st) {
-  const int rc = run_type(p, true, st);
-  if (rc || p.ws == nullptr) return rc;
-  ln_bwd_join_kernel<<<dim3((p.C + 31) / 32, 2), 256, 0, st>>>(p);
+  if (!valid(p) || p.blocks < 1) return 1;
+  const int rc = run_type(p, true, false, st);
+  if (rc || p.blocks == 1 || (p.dw == nullptr && p.db == nullptr)) return rc;
+  ln_bwd_join_kernel<<<dim3((p.C + 31) / 32, 2), 1024, 0, st>>>(p);
   return hipGetLastError() == hipSuccess ? 0 : 3;
 }

@@ -349,7 +349,7 @@ def check_norm(x, w, b, gy, eps=1e-3):
 @pytest.mark.parametrize("dt", [FF, BF, HF])
 @pytest.mark.parametrize("rows,C", [(1, 1), (1, 8), (3, 5), (70, 32), (33, 33), (130, 64), (17, 100), (9, 128), (50, 250),
                                     (5, 256), (40, 333), (6, 512), (10, 768), (3, 1024), (7, 1000), (3, 2048), (2, 2050),
-                                    (5, 4096), (3, 8192), (2, 8200), (2, 9001), (2, 16384), (3000, 32), (2100, 320)])
+                                    (5, 4096), (3, 8192), (2, 8191), (2, 4104), (1100, 1000), (3000, 32), (2100, 320)])
 def test_layer_norm_matches_definition(rows, C, dt):
     x = rnd((rows, C), dt, rows + C, 1.5, 0.5)
     check_norm(x, rnd((C,), FF, 1, 0.3, 1.0), rnd((C,), FF, 2, 0.3), rnd((rows, C), dt, 3))
