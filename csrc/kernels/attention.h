@@ -149,16 +149,16 @@ CFL_DEVICE s8v pack_b(const f16v& v, int s) {
 
 // 32 channels 32 * dt .. + 31 of one token row per lane pair (c, c + 32): four quads each, exchanged between the
 // halves so that a lane stores 16 contiguous bytes (lane half h: channels 16s + 8h .. + 7). rest: if given, what the
-// rounding took away, rounded itself.
+// rounding took away, rounded itself. zero: zeros are stored, whatever v holds.
 template <class T>
 CFL_DEVICE void store_row(bf16_t* row, const f16v& v, float mul, int dt, int D, int h, bool ok,
-                          bf16_t* rest = nullptr) {
+                          bf16_t* rest = nullptr, bool zero = false) {
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     unsigned w[4], x[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float a = v[8 * s + 2 * j] * mul, b = v[8 * s + 2 * j + 1] * mul;
+      const float a = zero ? 0.f : v[8 * s + 2 * j] * mul, b = zero ? 0.f : v[8 * s + 2 * j + 1] * mul;
       w[j] = T::pack2(a, b);
       x[j] = T::pack2(a - T::lo(w[j]), b - T::hi(w[j]));
     }
@@ -256,13 +256,18 @@ struct TileMask {
         int i0, i1, w0, w1;
         f(t, i0, i1, w0, w1);
         const int b0 = p.mask.rows > 1 ? i0 >> 5 : 0, b1 = p.mask.rows > 1 ? i1 >> 5 : 0;
-        for (int g = 0; g < heads; ++g)
-          for (int ib = b0; ib <= b1; ++ib)
-            for (int w = w0; w <= w1; ++w) {
-              const int k = p.mask.cls[((lead + g) * nib + ib) * p.mask.words + w];
-              any |= k != 0;
-              all &= k == 2;
-            }
+        // at most 128 queries and 128 keys: five class rows of two words, all of their loads under way together
+        for (int g = 0; g < heads; ++g) {
+          const uint8_t* c = p.mask.cls + (lead + g) * nib * p.mask.words;
+          int k[10];
+#pragma unroll
+          for (int j = 0; j < 10; ++j) k[j] = c[(int64_t)imin(b0 + (j >> 1), b1) * p.mask.words + (j & 1 ? w1 : w0)];
+#pragma unroll
+          for (int j = 0; j < 10; ++j) {
+            any |= k[j] != 0;
+            all &= k[j] == 2;
+          }
+        }
       }
       t8[t] = any ? (all ? 2 : 1) : 0;
     }

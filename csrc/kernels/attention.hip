@@ -352,15 +352,33 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnParams p) {
   const int64_t row = id / TPR;
   const int d = (int)(id % TPR) * 4;
   if (row >= rows) return;
-  float mn = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) mn = fmaxf(mn, p.ws_ml[(s * rows + row) * 2]);
-  const float ms = mn == -INFINITY ? 0.f : mn;
-  float l = 0.f, a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
-  for (int s = 0; s < p.splits; ++s) {
-    const float f = exp2_(p.ws_ml[(s * rows + row) * 2] - ms);
-    l += p.ws_ml[(s * rows + row) * 2 + 1] * f;
-    const float4 v = *reinterpret_cast<const float4*>(p.ws_o + (s * rows + row) * DP + d);
-    a0 += v.x * f; a1 += v.y * f; a2 += v.z * f; a3 += v.w * f;
+  // parts in order, eight at a time so that their loads are under way together
+  float mn = -INFINITY, l = 0.f, a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
+  for (int s0 = 0; s0 < p.splits; s0 += 8) {
+    float2 ml[8];
+    float4 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t at = imin(s0 + j, p.splits - 1) * rows + row;
+      ml[j] = *reinterpret_cast<const float2*>(p.ws_ml + at * 2);
+      v[j] = *reinterpret_cast<const float4*>(p.ws_o + at * DP + d);
+    }
+    float top = mn;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, s0 + j < p.splits ? ml[j].x : -INFINITY);
+    const float ms = top == -INFINITY ? 0.f : top, f0 = exp2_(mn - ms);
+    mn = top;
+    l *= f0; a0 *= f0; a1 *= f0; a2 *= f0; a3 *= f0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (s0 + j < p.splits) {
+        const float f = exp2_(ml[j].x - ms);
+        l = fmaf(ml[j].y, f, l);
+        a0 = fmaf(v[j].x, f, a0);
+        a1 = fmaf(v[j].y, f, a1);
+        a2 = fmaf(v[j].z, f, a2);
+        a3 = fmaf(v[j].w, f, a3);
+      }
   }
   const int bh = (int)(row / p.M), r = (int)(row - (int64_t)bh * p.M), b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const int i = fdiv(r, p.div_g), g = r - i * p.G;

@@ -537,25 +537,19 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
     const int key = wkey0 + 32 * u + c;
     bf16_t* ko = reinterpret_cast<bf16_t*>(p.dk.p) + b * p.dk.sb + key * p.dk.ss + hk * p.dk.sh;
     bf16_t* vo = reinterpret_cast<bf16_t*>(p.dv.p) + b * p.dv.sb + key * p.dv.ss + hk * p.dv.sh;
-    if (key >= len) {                                        // padding behind the image's keys
-#pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) dk[d][u][e] = dv[d][u][e] = 0.f;
-    }
     if (p.kv_splits > 1) {
       const int64_t part = ((int64_t)sp * bhn + bh) * p.Sk + key, half = (int64_t)p.kv_splits * bhn * p.Sk;
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        store_part<DP>(p.ws_kv + part * DP, dk[d][u], p.scale, d, h, key < p.Sk);
-        store_part<DP>(p.ws_kv + (half + part) * DP, dv[d][u], 1.f, d, h, key < p.Sk);
+        store_part<DP>(p.ws_kv + part * DP, dk[d][u], p.scale, d, h, key < len);
+        store_part<DP>(p.ws_kv + (half + part) * DP, dv[d][u], 1.f, d, h, key < len);
       }
       continue;
     }
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
-      if (p.dk.p) store_row<T>(ko, dk[d][u], p.scale, d, p.D, h, key < p.Sk);
-      if (p.dv.p) store_row<T>(vo, dv[d][u], 1.f, d, p.D, h, key < p.Sk);
+      if (p.dk.p) store_row<T>(ko, dk[d][u], p.scale, d, p.D, h, key < p.Sk, nullptr, key >= len);
+      if (p.dv.p) store_row<T>(vo, dv[d][u], 1.f, d, p.D, h, key < p.Sk, nullptr, key >= len);
     }
   }
 }
@@ -563,17 +557,18 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
 // gradients of a token tensor from the parts of `splits` blocks: one thread per 4 channels, parts in order
 template <class T, int DP>
 __global__ __launch_bounds__(256) void attn_sum_kernel(const float* ws, int splits, AttnTensor out, int B, int H, int G,
-                                                       int rows, int D, FastDiv div_g) {
+                                                       int rows, int D, FastDiv div_g, const int* lengths) {
   constexpr int TPR = DP / 4;
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (int64_t)B * H * rows, row = id / TPR;
   const int d = (int)(id % TPR) * 4;
   if (row >= all || d >= D) return;
+  const int bh = (int)(row / rows), r = (int)(row - (int64_t)bh * rows), b = bh / H, hk = bh - b * H;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < splits; ++s) {
+  const int n = lengths && r >= lengths[b] ? 0 : splits;    // keys behind the image's: nothing was written
+  for (int s = 0; s < n; ++s) {
     const float4 v = *reinterpret_cast<const float4*>(ws + (s * all + row) * DP + d);
     a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
   }
-  const int bh = (int)(row / rows), r = (int)(row - (int64_t)bh * rows), b = bh / H, hk = bh - b * H;
   const int i = fdiv(r, div_g), g = r - i * G;
   bf16_t* o = reinterpret_cast<bf16_t*>(out.p) + b * out.sb + i * out.ss + (hk * G + g) * out.sh + d;
   *reinterpret_cast<uint2*>(o) = make_uint2(T::pack2(a.x, a.y), T::pack2(a.z, a.w));
@@ -585,7 +580,7 @@ void bwd(const AttnParams& p, hipStream_t st) {
   attn_dq_kernel<T, DP, 1, KIND><<<(unsigned)((p.M + 127) / 128 * bhn * p.splits), 256, 0, st>>>(p);
   if (p.splits > 1 && p.dq.p)
     attn_sum_kernel<T, DP><<<(unsigned)((bhn * p.M * (DP / 4) + 255) / 256), 256, 0, st>>>(
-        p.ws_o, p.splits, p.dq, p.B, p.Hkv, p.G, p.M, p.D, p.div_g);
+        p.ws_o, p.splits, p.dq, p.B, p.Hkv, p.G, p.M, p.D, p.div_g, nullptr);
   if ((p.dk.p == nullptr && p.dv.p == nullptr) || p.Sk == 0) return;
   constexpr bool VL = DP >= 96;
   attn_dkv_kernel<T, DP, 1, DP == 128 ? 32 : 64, VL, KIND>
@@ -595,10 +590,10 @@ void bwd(const AttnParams& p, hipStream_t st) {
     const unsigned grid = (unsigned)((n * (DP / 4) + 255) / 256);
     const FastDiv one = fast_div(1);
     if (p.dk.p)
-      attn_sum_kernel<T, DP><<<grid, 256, 0, st>>>(p.ws_kv, p.kv_splits, p.dk, p.B, p.Hkv, 1, p.Sk, p.D, one);
+      attn_sum_kernel<T, DP><<<grid, 256, 0, st>>>(p.ws_kv, p.kv_splits, p.dk, p.B, p.Hkv, 1, p.Sk, p.D, one, p.lengths);
     if (p.dv.p)
       attn_sum_kernel<T, DP><<<grid, 256, 0, st>>>(p.ws_kv + p.kv_splits * n * DP, p.kv_splits, p.dv, p.B, p.Hkv, 1,
-                                                   p.Sk, p.D, one);
+                                                   p.Sk, p.D, one, p.lengths);
   }
 }
 
@@ -613,12 +608,12 @@ void bwd_d(const AttnParams& p, hipStream_t st) {
 }  // namespace
 
 // Blocks that share a row block's keys (dq) and a key block's rows (dk, dv): as attn_splits, up to two blocks a CU, or
-// four for causal dk, dv, whose blocks are as unequal as their keys (2 images, 16 heads that share 2, 8,192 tokens, 128
+// four for dk, dv where blocks differ (causal, 2 images, 16 heads that share 2, 8,192 tokens, 128
 // channels: 2,862 / 2,041 / 2,053 us for 512 / 1,024 / 2,048 blocks); at least four tiles each.
-void attn_bwd_splits(int B, int Hkv, int M, int Sk, int causal, int& splits, int& kv_splits) {
+void attn_bwd_splits(int B, int Hkv, int M, int Sk, bool uneven, int& splits, int& kv_splits) {
   const int64_t bhn = (int64_t)B * Hkv, qb = (M + 127) / 128 * bhn, kb = std::max<int64_t>(1, (Sk + 127) / 128 * bhn);
   splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / qb, (Sk + 63) / 64 / 4));
-  kv_splits = (int)std::max<int64_t>(1, std::min<int64_t>((causal ? 1024 : 512) / kb, (M + 63) / 64 / 4));
+  kv_splits = (int)std::max<int64_t>(1, std::min<int64_t>((uneven ? 1024 : 512) / kb, (M + 63) / 64 / 4));
 }
 
 int attn_bwd(const AttnParams& p, hipStream_t st) {
