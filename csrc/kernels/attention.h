@@ -64,13 +64,19 @@ CFL_DEVICE float other_half(float v) {
 }
 
 // LDS image of a tile of token rows, DP 16-bit values each: row-major without padding (an LDS-DMA load writes 16
-// bytes a lane, lanes in order), the 16-byte chunks of a row permuted by its index. Eight rows in a row then hold a
-// given chunk in eight different 16-byte bank groups (fragment reads, ds_read_b128), and four rows in a row hold a
-// given 64-byte quarter alternately in both halves of the 128-byte bank line (transposing reads, ds_read_b64_tr_b16).
+// bytes a lane, lanes in order), the 16-byte chunks of a row permuted by its index. 64 banks of 4 bytes serve a 256-byte
+// line per cycle, so that
+//   - a fragment read (ds_read_b128, 16 lanes a cycle: rows that differ modulo 16, one chunk) needs 16 rows to hold a
+//     chunk in the 16 places of a line,
+//   - a transposing read (ds_read_b64_tr_b16, 32 lanes a cycle: rows 4a .. 4a + 3, one 64-byte quarter) needs four rows in
+//     a row to hold a quarter in the four quarters of a line.
+// Rows of 64 and 192 bytes alternate the quarters by themselves. (A permutation made for lines of 128 bytes left half of
+// the LDS cycles to conflicts.)
 template <int DP>
 CFL_DEVICE int swz(int row) {
-  if (DP % 64 != 0) return (row >> 1) & 3;             // rows of 64 or 192 bytes alternate the halves by themselves
-  return ((row & 1) << 2) | ((row >> 1) & 3);
+  if (DP == 128) return ((row & 3) << 2) | ((row >> 2) & 3);
+  if (DP == 64) return ((row & 2) << 1) | ((row >> 2) & 3);
+  return (row >> 2) & 3;
 }
 template <int DP>
 CFL_DEVICE int lds_at(int row, int chunk) { return row * DP + ((chunk ^ swz<DP>(row)) << 3); }
@@ -88,13 +94,24 @@ CFL_DEVICE s4v tr4(const bf16_t* p) {
 }
 
 // A operand of a product that reduces over token rows: operand row = channel 32 * dt + c, slots = token rows
-// row0 + {0-3, 8-11} + 4h (row0 a multiple of 16)
+// row0 + {0-3, 8-11} + 4h (row0 a multiple of 16). Rows 16 apart are permuted alike, so a lane's addresses are two per
+// channel tile (TransAt), formed once, and offsets that the compiler puts into the instructions.
 template <int DP>
-CFL_DEVICE s8v frag_t(const bf16_t* tile, int row0, int dt, int lane) {
-  const int p = lane & 15, row = row0 + ((lane >> 5) << 2) + (p >> 2);
-  const int col = 32 * dt + (lane & 16) + ((p & 3) << 2);
-  const s4v a = tr4(tile + lds_at<DP>(row, col >> 3) + (col & 7));
-  const s4v b = tr4(tile + lds_at<DP>(row + 8, col >> 3) + (col & 7));
+struct TransAt {
+  int at[DP / 32][2];
+  CFL_DEVICE explicit TransAt(int lane) {
+    const int p = lane & 15, row = ((lane >> 5) << 2) + (p >> 2);
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) {
+      const int col = 32 * dt + (lane & 16) + ((p & 3) << 2);
+      at[dt][0] = lds_at<DP>(row, col >> 3) + (col & 7);
+      at[dt][1] = lds_at<DP>(row + 8, col >> 3) + (col & 7);
+    }
+  }
+};
+template <int DP>
+CFL_DEVICE s8v frag_t(const bf16_t* rows, const TransAt<DP>& t, int dt) {
+  const s4v a = tr4(rows + t.at[dt][0]), b = tr4(rows + t.at[dt][1]);
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
@@ -215,6 +232,13 @@ CFL_DEVICE u4v rsrc(const void* base) {
 }
 
 CFL_DEVICE int fdiv(int x, const FastDiv& f) { return fdiv32(x, f); }
+
+// max of a value and the one 32 lanes away
+CFL_DEVICE float max_halves(float v) {
+  const unsigned u = __builtin_bit_cast(unsigned, v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
+}
 
 // Which of `n` blocks of an (image, key head), which of bhn of those and which of `splits` parts this workgroup is.
 // Where all blocks have the same work, XCD by XCD: the blocks that read one head's tokens share an L2 (16 heads, 4,096

@@ -128,6 +128,7 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
   float m[QT], l[QT];
   const float sc = p.scale * LOG2E;
   const int fo = lds_at<DP>(c, h);
+  const TransAt<DP> ta(lane);
   auto walk = [&](auto safe) {
     constexpr bool SAFE = decltype(safe)::value;
 #pragma unroll
@@ -140,7 +141,7 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
         for (int e = 0; e < 16; ++e) acc[d][t][e] = 0.f;
     }
 
-    int t = next(t0), buf = 0;
+    int t = next(t0);
     if (t < t1) {
       if (MASK) words(t);
       issue(t, 0);
@@ -148,7 +149,9 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
     wait_vm();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    while (t < t1) {
+    // the tile in buffer B. Taking turns with a constant buffer leaves all LDS offsets to the instructions.
+    auto step = [&](auto B) {
+      const int buf = B;
       const bool part = MASK && tm.part;
       const int tn = next(t + 1);
       unsigned long long cur[QT];
@@ -207,7 +210,7 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
           for (int k = 0; k < NK; ++k)
 #pragma unroll
             for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[k][u][e]);
-          mx = fmaxf(mx, other_half(mx)) * sc;
+          mx = max_halves(mx) * sc;
           if (__any(mx > m[u] + SLACK)) {
             // only the rows that need it: what a row rounds does not depend on the rows next to it
             const bool up = mx > m[u] + SLACK;
@@ -237,7 +240,7 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
         for (int ks = 0; ks < 2 * NK; ++ks)
 #pragma unroll
           for (int d = 0; d < ND; ++d) {
-            s8v a = frag_t<DP>(sv, 16 * ks, d, lane);
+            s8v a = frag_t<DP>(sv + 16 * ks * DP, ta, d);
             if constexpr (SAFE) {
               s8v pos, neg;
               __builtin_amdgcn_sched_barrier(0);           // few registers matter here, not speed
@@ -252,8 +255,12 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      buf ^= 1;
       t = tn;
+    };
+    while (t < t1) {
+      step(std::integral_constant<int, 0>{});
+      if (t >= t1) break;
+      step(std::integral_constant<int, 1>{});
     }
 
   };
@@ -271,46 +278,45 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
   for (int u = 0; u < QT; ++u) l[u] += other_half(l[u]);
 
   if constexpr (WK > 1) {
-    // join the waves that share rows: every wave's (m, l) and accumulators through LDS, wave w finishes the channel
-    // tiles w, w + WK, ...
+    // join the waves that share rows: the first one collects the others' (m, l) and accumulators through LDS
     static_assert(QT == 1 && WR == 1, "key-split waves hold one row tile");
-    constexpr int SEG = ND * 1024 + 128;                   // floats per wave
-      static_assert(WK * SEG * 4 <= (int)sizeof(smem), "LDS of the join");
+    constexpr int SEG = ND * 1024 + 64;                     // floats per wave
+    static_assert((WK - 1) * SEG * 4 <= (int)sizeof(smem), "LDS of the join");
     float* sf = reinterpret_cast<float*>(smem);
-    float* mine = sf + wk * (ND * 1024);
-    float* ml = sf + WK * ND * 1024;
+    if (wk > 0) {
+      float* mine = sf + (wk - 1) * SEG;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mine[(d * 16 + e) * 64 + lane] = acc[d][0][e];
+      if (h == 0) {
+        mine[ND * 1024 + 2 * c] = m[0];
+        mine[ND * 1024 + 2 * c + 1] = l[0];
+      }
+    }
+    __syncthreads();
+    if (wk > 0) return;
+    float mn = m[0], f[WK];
+#pragma unroll
+    for (int w = 1; w < WK; ++w) mn = fmaxf(mn, sf[(w - 1) * SEG + ND * 1024 + 2 * c]);
+    const float ms = mn == -INFINITY ? 0.f : mn;
+    f[0] = exp2_(m[0] - ms);
+    l[0] *= f[0];
+#pragma unroll
+    for (int w = 1; w < WK; ++w) {
+      f[w] = exp2_(sf[(w - 1) * SEG + ND * 1024 + 2 * c] - ms);
+      l[0] = fmaf(sf[(w - 1) * SEG + ND * 1024 + 2 * c + 1], f[w], l[0]);
+    }
+    m[0] = mn;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) mine[(d * 16 + e) * 64 + lane] = acc[d][0][e];
-    if (h == 0) {
-      ml[(wk * 32 + c) * 2] = m[0];
-      ml[(wk * 32 + c) * 2 + 1] = l[0];
-    }
-    __syncthreads();
-    float mn = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < WK; ++w) mn = fmaxf(mn, ml[(w * 32 + c) * 2]);
-    const float ms = mn == -INFINITY ? 0.f : mn;
-    float f[WK], ls = 0.f;
-#pragma unroll
-    for (int w = 0; w < WK; ++w) {
-      f[w] = exp2_(ml[(w * 32 + c) * 2] - ms);
-      ls += ml[(w * 32 + c) * 2 + 1] * f[w];
-    }
-    m[0] = mn;
-    l[0] = ls;
-#pragma unroll
-    for (int d = 0; d < ND; ++d) {
-      if (d % WK != wk) continue;
-#pragma unroll
       for (int e = 0; e < 16; ++e) {
-        float a = 0.f;
+        float x = acc[d][0][e] * f[0];
 #pragma unroll
-        for (int w = 0; w < WK; ++w) a += sf[(w * ND * 16 + d * 16 + e) * 64 + lane] * f[w];
-        acc[d][0][e] = a;
+        for (int w = 1; w < WK; ++w) x = fmaf(sf[(w - 1) * SEG + (d * 16 + e) * 64 + lane], f[w], x);
+        acc[d][0][e] = x;
       }
-    }
   }
 
 #pragma unroll
@@ -322,10 +328,9 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
       const int64_t part = (int64_t)sp * bhn * p.M + row;
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        if (WK > 1 && d % WK != wk) continue;
         store_part<DP>(p.ws_o + part * DP, acc[d][u], 1.f, d, h, ok);
       }
-      if (ok && h == 0 && wk == 0) {
+      if (ok && h == 0) {
         p.ws_ml[part * 2] = m[u];
         p.ws_ml[part * 2 + 1] = l[u];
       }
@@ -336,10 +341,9 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
     bf16_t *o = reinterpret_cast<bf16_t*>(p.o.p) + at, *rest = p.o_rest ? p.o_rest + at : nullptr;
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
-      if (WK > 1 && d % WK != wk) continue;
       store_row<T>(o, acc[d][u], inv, d, p.D, h, ok, rest);
     }
-    if (ok && h == 0 && wk == 0 && p.lse2)
+    if (ok && h == 0 && p.lse2)
       p.lse2[row] = l[u] == 0.f ? INFINITY : m[u] + __builtin_amdgcn_logf(l[u]);
   }
 }
@@ -460,11 +464,12 @@ int attn_mask_bits(const AttnMaskArgs& a, hipStream_t st) {
 }
 
 // Blocks that share the keys of a row block: enough for two blocks a CU where there are few row blocks, at least four
-// tiles each.
+// tiles each. (Blocks of 64 rows with two waves along the keys instead, for such grids, were slower: 4 images x 8 heads
+// x 1,600 tokens of 64 channels 43 us against 40.)
 int attn_splits(int B, int Hkv, int M, int Sk) {
   const int64_t blocks = (int64_t)((M + 127) / 128) * B * Hkv;
-  const int tiles = M <= FEW_ROWS ? (Sk + 127) / 128 : (Sk + 63) / 64;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(512 / blocks, tiles / 4));
+  const int tile = M <= FEW_ROWS ? 128 : 64;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(512 / blocks, (Sk + tile - 1) / tile / 4));
 }
 
 int attn_fwd(const AttnParams& p, hipStream_t st) {

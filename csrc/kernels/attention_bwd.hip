@@ -72,7 +72,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
       gf[t][kk] = __builtin_bit_cast(s8v, wg);
     }
     delta[t] = dl + other_half(dl);
-    if (ok && h == 0 && sp == 0) p.delta[(int64_t)bh * p.M + r] = delta[t];
+    if (ok && h == 0 && sp == 0) p.delta[(int64_t)bh * p.M + r] = -delta[t];
   }
   if (p.dq.p == nullptr) return;
 
@@ -131,6 +131,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
 
   f16v acc[ND][QT];
   const float sc = p.scale * LOG2E;
+  const TransAt<DP> ta(lane);
   auto walk = [&](auto safe) {
     constexpr bool SAFE = decltype(safe)::value;
 #pragma unroll
@@ -140,7 +141,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[d][t][e] = 0.f;
 
-    int t = next(t0), buf = 0;
+    int t = next(t0);
     if (t < t1) {
       if (MASK) words(t);
       issue(t, 0);
@@ -148,7 +149,9 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
     wait_vm();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    while (t < t1) {
+    // the tile in buffer B. Taking turns with a constant buffer leaves all LDS offsets to the instructions.
+    auto step = [&](auto B) {
+      const int buf = B;
       const int key0 = t * KT;
       const bool part = MASK && tm.part;
       const int tn = next(t + 1);
@@ -174,7 +177,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
 #pragma unroll
           for (int u = 0; u < QT; ++u) {
             nd[u] = -delta[u];
-            asm volatile("" : "+v"(nd[u]));                // or 16 copies of it stay in registers
+            if (DP == 128) asm volatile("" : "+v"(nd[u])); // or 16 copies of it stay in registers
           }
 #pragma unroll
           for (int u = 0; u < QT; ++u)
@@ -224,7 +227,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
           for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
-              s8v a = frag_t<DP>(sk, 32 * k + 16 * ks, d, lane);
+              s8v a = frag_t<DP>(sk + (32 * k + 16 * ks) * DP, ta, d);
               if constexpr (SAFE) {                          // an allowed key that is not finite shows in its scores
                 s8v pos, neg;
                 __builtin_amdgcn_sched_barrier(0);         // few registers matter here, not speed
@@ -238,8 +241,12 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      buf ^= 1;
       t = tn;
+    };
+    while (t < t1) {
+      step(std::integral_constant<int, 0>{});
+      if (t >= t1) break;
+      step(std::integral_constant<int, 1>{});
     }
   };
   walk(std::false_type{});
@@ -277,7 +284,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
   constexpr bool MASK = KIND == ATTN_MASK;
   const bool causal = KIND == ATTN_CAUSAL || (MASK && p.causal);
   __shared__ __attribute__((aligned(1024))) bf16_t smem[4 * TILE + VTILE];
-  __shared__ __attribute__((aligned(256))) float sstat[2][2][64];      // [buffer][lse2, delta][row]
+  __shared__ __attribute__((aligned(256))) float sstat[2][2][64];      // [buffer][lse2, -delta][row]
 
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, h = lane >> 5;
@@ -386,6 +393,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
 
   f16v dk[ND][KQ], dv[ND][KQ];
   const float sc = p.scale * LOG2E;
+  const TransAt<DP> ta(lane);
   auto walk = [&](auto safe) {
     constexpr bool SAFE = decltype(safe)::value;
 #pragma unroll
@@ -395,7 +403,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) dk[d][u][e] = dv[d][u][e] = 0.f;
 
-    int t = t1 > t0 ? next(t0) : t0, buf = 0;
+    int t = t1 > t0 ? next(t0) : t0;
     if (t < t1) {
       if (MASK) words(t);
       issue(t, 0);
@@ -403,7 +411,9 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
     wait_vm();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    while (t < t1) {
+    // the tile in buffer B. Taking turns with a constant buffer leaves all LDS offsets to the instructions.
+    auto step = [&](auto B) {
+      const int buf = B;
       const bool part = MASK && tm.part;
       const int tn = next(t + 1);
       if (MASK) {
@@ -434,7 +444,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               s[u][4 * q + j] = 0.f;
-              dp[u][4 * q + j] = -y[j];                    // the product sums dp - delta
+              dp[u][4 * q + j] = y[j];                     // the product sums dp - delta
             }
           }
 #pragma unroll
@@ -491,7 +501,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
           for (int d = 0; d < ND; ++d) {
-            s8v a = frag_t<DP>(sg, 32 * n + 16 * ks, d, lane);
+            s8v a = frag_t<DP>(sg + (32 * n + 16 * ks) * DP, ta, d);
             if constexpr (SAFE) {
               s8v pos, neg;
               __builtin_amdgcn_sched_barrier(0);           // few registers matter here, not speed
@@ -506,7 +516,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
           for (int d = 0; d < ND; ++d) {
-            s8v a = frag_t<DP>(sq, 32 * n + 16 * ks, d, lane);
+            s8v a = frag_t<DP>(sq + (32 * n + 16 * ks) * DP, ta, d);
             if constexpr (SAFE) {                            // an allowed query that is not finite shows in its scores
               s8v pos, neg;
               __builtin_amdgcn_sched_barrier(0);           // few registers matter here, not speed
@@ -519,8 +529,12 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      buf ^= 1;
       t = tn;
+    };
+    while (t < t1) {
+      step(std::integral_constant<int, 0>{});
+      if (t >= t1) break;
+      step(std::integral_constant<int, 1>{});
     }
   };
   walk(std::false_type{});
@@ -582,8 +596,7 @@ void bwd(const AttnParams& p, hipStream_t st) {
     attn_sum_kernel<T, DP><<<(unsigned)((bhn * p.M * (DP / 4) + 255) / 256), 256, 0, st>>>(
         p.ws_o, p.splits, p.dq, p.B, p.Hkv, p.G, p.M, p.D, p.div_g, nullptr);
   if ((p.dk.p == nullptr && p.dv.p == nullptr) || p.Sk == 0) return;
-  constexpr bool VL = DP >= 96;
-  attn_dkv_kernel<T, DP, 1, DP == 128 ? 32 : 64, VL, KIND>
+  attn_dkv_kernel<T, DP, 1, DP == 128 ? 32 : 64, DP >= 96, KIND>
       <<<(unsigned)((p.Sk + 127) / 128 * bhn * p.kv_splits), 256, 0, st>>>(p);
   if (p.kv_splits > 1) {
     const int64_t n = bhn * p.Sk;

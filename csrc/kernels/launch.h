@@ -640,7 +640,7 @@ struct AttnParams {
   bf16_t* o_rest;                   // o before its rounding less o, laid out like o; kept for the backward (or nullptr)
   AttnTensor go, dq, dk, dv;        // backward
   float* lse2;                      // [B][Hkv][M] log2 of the row's exp2 sum (+inf: empty row); saved for the backward
-  float* delta;                     // [B][Hkv][M] workspace of the backward
+  float* delta;                     // [B][Hkv][M] -sum(do o), workspace of the backward
   AttnMask mask;
   const int* lengths;               // [B] valid keys or nullptr
   int B, Sq, Sk, Hq, Hkv, G, D, M;  // M = Sq * G

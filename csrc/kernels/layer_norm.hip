@@ -71,12 +71,18 @@ CFL_DEVICE float lane_sum(float v) {
   return v;
 }
 
+// sum / n by the reciprocal, corrected once: the quotient of a sum of equal values is that value
+CFL_DEVICE float mean_of(float sum, float n, float inv) {
+  const float m = sum * inv;
+  return fmaf(fmaf(-m, n, sum), inv, m);
+}
+
 // What the statistics need that is the same for every row: 1 / C and, for a row of several waves, the columns of this
 // wave and of each.
 template <int LPR>
 struct RowShape {
   static constexpr int W = LPR > 64 ? LPR / 64 : 1;
-  float inv, own;                // 1 / C; 1 / columns of this wave (0: none)
+  float inv, own, n;             // 1 / C; 1 / columns of this wave (0: none); those columns
   float part[W];                 // columns of each wave
 };
 template <int LPR, int NV, int V>
@@ -84,6 +90,7 @@ CFL_DEVICE RowShape<LPR> row_shape(int C) {
   RowShape<LPR> s;
   s.inv = 1.f / (float)C;
   s.own = s.inv;
+  s.n = (float)C;
   if constexpr (LPR > 64) {
 #pragma unroll
     for (int u = 0; u < LPR / 64; ++u) {
@@ -91,7 +98,10 @@ CFL_DEVICE RowShape<LPR> row_shape(int C) {
 #pragma unroll
       for (int k = 0; k < NV; ++k) n += imax(0, imin(C - (k * LPR + 64 * u) * V, 64 * V));
       s.part[u] = (float)n;
-      if (u == (int)(threadIdx.x % LPR) >> 6) s.own = n > 0 ? 1.f / (float)n : 0.f;
+      if (u == (int)(threadIdx.x % LPR) >> 6) {
+        s.own = n > 0 ? 1.f / (float)n : 0.f;
+        s.n = (float)n;
+      }
     }
   }
   return s;
@@ -110,7 +120,7 @@ CFL_DEVICE float center(float (*x)[V], const int* col, int C, float eps, const R
   for (int k = 0; k < NV; ++k)
 #pragma unroll
     for (int j = 0; j < V; ++j) s += x[k][j];
-  const float mw = lane_sum<LPR>(s) * sh.own;
+  const float mw = mean_of(lane_sum<LPR>(s), sh.n, sh.own);
   float q = 0.f;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
@@ -134,7 +144,7 @@ CFL_DEVICE float center(float (*x)[V], const int* col, int C, float eps, const R
       w[u] = red[u];
       mu = fmaf(w[u].x, sh.part[u], mu);
     }
-    mu *= sh.inv;
+    mu = mean_of(mu, (float)C, sh.inv);
     q = 0.f;
 #pragma unroll
     for (int u = 0; u < W; ++u) q += fmaf(sh.part[u] * (w[u].x - mu), w[u].x - mu, w[u].y);
@@ -269,12 +279,14 @@ __global__ __launch_bounds__(NT) void ln_bwd_kernel(const LayerNormParams p) {
         s1 += red2[par][gr][u].y;
       }
     }
-    const float m0 = -s0 * sh.inv * rs, m1 = -s1 * sh.inv * rs;
+    // the mean taken from dy w before anything is scaled: a row of one column, or of equal ones, gives 0 and not the
+    // rounding of a product
+    const float m0 = s0 * sh.inv, m1 = s1 * sh.inv;
     E* yr = reinterpret_cast<E*>(p.y) + r * p.C;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[k][j] = fmaf(x[k][j], m1, fmaf(g[k][j], rs, m0));
+      for (int j = 0; j < V; ++j) x[k][j] = rs * fmaf(x[k][j], -m1, g[k][j] - m0);
       if (ok && col[k] < p.C) store_v<TYPE, V>(yr + col[k], x[k]);
     }
   }

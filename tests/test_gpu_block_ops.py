@@ -158,6 +158,21 @@ def test_attention_matches_definition(shape, causal, dt):
 
 
 @pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("kind", ["plain", "causal", "mask", "lengths"])
+@pytest.mark.parametrize("D", [32, 64, 80, 128])
+def test_attention_many_blocks(D, kind, dt):
+    """Enough (image, head)s for the blocks of 128 rows and 128 keys that large calls take."""
+    B, Hq, Hkv, Sq, Sk = 20, 28, 28, 140, 150
+    g = torch.Generator().manual_seed(17)
+    kw = {}
+    if kind == "mask":
+        kw["mask"] = (torch.rand(1, 1, Sq, Sk, generator=g) < 0.5).to(DEV)
+    elif kind == "lengths":
+        kw["lengths"] = torch.randint(0, Sk + 1, (B,), generator=g, dtype=torch.int32).to(DEV)
+    check_attention(*qkvg(B, Sq, Sk, Hq, Hkv, D, dt), causal=kind == "causal", **kw)
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("shape", [(4, 70, 70, 4, 2, 64), (4, 1, 700, 4, 4, 32), (4, 150, 260, 2, 2, 128)])
 def test_attention_lengths(shape, causal, dt):
@@ -380,8 +395,17 @@ def test_layer_norm_large_mean_and_constant_rows():
     """The variance is of x - mean: a mean a thousand times the spread loses nothing but its own rounding."""
     x = rnd((40, 256), FF, 0, 1.0, 1000.0)
     check_norm(x, None, None, rnd((40, 256), FF, 1))
-    x = torch.full((4, 64), 3.25, device=DEV)
-    assert not ops.layer_norm(x).any()
+    for C in (1, 3, 64, 100, 333, 700, 5000):
+        for dt in (FF, BF, HF):
+            x = torch.full((4, C), 3.25, dtype=dt, device=DEV).requires_grad_()
+            y = ops.layer_norm(x)
+            assert not y.any()
+            # equal gradients: nothing is left of them (a row of one column never keeps any)
+            g = rnd((4, 1), dt, C).expand(4, C).contiguous()
+            (dx,) = torch.autograd.grad(y, x, g)
+            assert C > 1 or not dx.any()
+            tol = 64 * U32 * float(g.abs().max()) * math.sqrt(1e3) * 2
+            assert float(dx.abs().max()) <= tol
 
 
 def test_layer_norm_frozen_inputs_and_empty_rows():
