@@ -595,7 +595,6 @@ at::Tensor rotary(const at::Tensor& x, const at::Tensor& pos, const std::vector<
                          pos.size(2) == S),
                     "rotary: positions must be (", A, ", ", S, ") or (", A, ", ", B, ", ", S, "), got ", pos.sizes());
   TORCH_CHECK_VALUE(!pos.requires_grad(), "rotary: positions have no gradient");
-  TORCH_CHECK_VALUE(x.numel() / 2 < (int64_t)1 << 31 || x.size(3) % 8 == 0, "rotary: too large: x ", x.sizes());
   TORCH_CHECK(x.is_cuda(), "rotary: x must be a device tensor");
   check_device(pos, x, "rotary: positions");
   pl.theta = theta;

@@ -166,6 +166,8 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
       if (key0 < wlast) {
         const bf16_t* sk = smem + buf * 2 * TILE + wk * KW * DP;
         const bf16_t* sv = sk + TILE;
+        // a wave in its products goes first, those in their softmax fill in (2 % here, nothing in the backward kernels)
+        __builtin_amdgcn_s_setprio(1);
         f16v s[NK][QT];
 #pragma unroll
         for (int k = 0; k < NK; ++k)
@@ -202,6 +204,7 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
               for (int e = 0; e < 16; ++e) s[k][u][e] = (e & 3) + 8 * (e >> 2) < left ? s[k][u][e] : -INFINITY;
             }
         }
+        __builtin_amdgcn_s_setprio(0);
         s8v pb[QT][2 * NK];
 #pragma unroll
         for (int u = 0; u < QT; ++u) {
@@ -236,6 +239,7 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
           }
           l[u] += sum;
         }
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int ks = 0; ks < 2 * NK; ++ks)
 #pragma unroll
@@ -252,6 +256,7 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
             for (int u = 0; u < QT; ++u) acc[d][u] = T::mma(a, pb[u][ks], acc[d][u]);
           }
       }
+      __builtin_amdgcn_s_setprio(0);
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
