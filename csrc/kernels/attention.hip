@@ -7,6 +7,15 @@
 //
 // Rounding: scores, maximum, sum and output accumulate in fp32. P is rounded to the inputs' type (relative error at most
 // half a step per term, independent from key to key), the output once.
+// Split. Four waves own 32 rows each and share the tiles (64 keys); up to 32 rows in all, the waves split a tile's keys
+// instead and join through LDS. Few row blocks: blocks share a walk (attn_splits) and a second launch joins the parts.
+// 256 registers, two waves a SIMD or more: at 512 the compiler puts the first product's result into accumulation
+// registers and copies every score (16 heads x 4,096 tokens x 128 channels: 479 us against 294).
+// Bound. Up to 64 channels by the vector unit (75 % busy; 32 scores cost a lane 32 exponentials of 8 cycles and 128 other
+// operations, the products half of that time), at 128 channels by both it and the matrix cores; no LDS bank conflicts.
+// 2 images x 16 heads x 4,096 tokens: 128 channels 283 us = 972 TFLOP/s; 4 images, 64 channels 314 us = 875 (a library
+// product of 8,192^3 reaches 1,213). One query of 64 (image, head)s over 4,096 keys of 32 channels: 8.3 us + 2.3 us to
+// join = 3.2 TB/s.
 // Rows that may attend nothing are 0 and their saved lse2 is +inf (exp2(s - inf) = 0 in the backward pass).
 #include <algorithm>
 
