@@ -776,3 +776,107 @@ def test_attention_mask_past_the_table_of_tiles():
     q, k, v, go = qkvg(1, many, 40, 1, 1, 8, BF)
     mask = (torch.rand(many, 40, generator=torch.Generator().manual_seed(3)) < 0.5).to(DEV)
     check_attention(q, k, v, go, mask=mask)
+
+
+# ------------------------------------------------------------------------------- walks split over blocks, calls at once
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("kind", ["lengths", "lengths causal", "mask", "mask causal"])
+@pytest.mark.parametrize("shape", [(3, 70, 1500, 2, 1, 64), (3, 900, 900, 2, 2, 96), (3, 1, 4000, 4, 2, 32),
+                                   (3, 1400, 90, 3, 1, 128)])
+def test_attention_split_walks(shape, kind, dt):
+    """Few row or key blocks: several blocks share a walk, some of whose parts are empty. Dead keys hold NaN."""
+    B, Sq, Sk = shape[:3]
+    q, k, v, go = qkvg(*shape, dt)
+    kw = {"causal": "causal" in kind}
+    n = [0, Sk // 2, Sk]
+    if "lengths" in kind:
+        kw["lengths"] = torch.tensor(n, dtype=torch.int32, device=DEV)
+    else:
+        g = torch.Generator().manual_seed(23)
+        m = (torch.rand(B, 1, 1, Sk, generator=g) < 0.7) & (torch.arange(Sk) < torch.tensor(n)[:, None, None, None])
+        kw["mask"] = m.to(DEV)
+        dead = ~m[:, 0, 0].to(DEV)
+        k[dead] = math.nan
+        v[dead] = math.inf
+    if "lengths" in kind:
+        for b in range(B):
+            k[b, n[b]:] = math.inf
+            v[b, n[b]:] = math.nan
+    check_attention(q, k, v, go, **kw)
+
+
+def test_gradient_of_a_sum_is_that_of_ones():
+    """An expanded gradient (strides of 0) is read as what it stands for."""
+    q, k, v, _ = qkvg(2, 50, 60, 2, 2, 32, BF)
+    x, pos = rnd((2, 50, 2, 32), BF, 4), torch.arange(50, device=DEV)[None]
+    w = rnd((32,), FF, 5)
+    for f, ins in ((lambda *t: ops.attention(*t), (q, k, v)), (lambda t: ops.rotary(t, pos, (32,)), (x,)),
+                   (lambda t, u: ops.layer_norm(t, u), (x, w))):
+        ins = [t.detach().requires_grad_() for t in ins]
+        a = torch.autograd.grad(f(*ins).sum(), ins)
+        out = f(*ins)
+        b = torch.autograd.grad(out, ins, torch.ones_like(out))
+        for s, t in zip(a, b):
+            assert torch.equal(s, t)
+
+
+def test_calls_at_once_on_two_streams_and_threads():
+    """Workspaces are a call's own: two threads on streams of their own get what one gets."""
+    import threading
+    cases = []
+    for seed, shape in ((1, (1, 30, 3000, 2, 2, 64)), (7, (2, 600, 500, 2, 1, 32))):
+        q, k, v, go = qkvg(*shape, BF, seed)
+        x, w, gy = rnd((3000, 96), BF, seed), rnd((96,), FF, seed), rnd((3000, 96), BF, seed + 1)
+
+        def run(q=q, k=k, v=v, go=go, x=x, w=w, gy=gy):
+            ins = [t.detach().requires_grad_() for t in (q, k, v, x, w)]
+            out = [ops.attention(*ins[:3], causal=True), ops.layer_norm(*ins[3:])]
+            return [t.detach() for t in out] + list(torch.autograd.grad(out, ins, [go, gy]))
+        cases.append((run, run()))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(run, want):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got = run()
+            s.synchronize()
+        bad.extend(n for n, (a, b) in enumerate(zip(got, want)) if not torch.equal(a, b))
+
+    ts = [threading.Thread(target=work, args=c) for c in cases]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join(60)
+        assert not t.is_alive()
+    assert not bad
+
+
+def test_layer_norm_is_the_same_every_time():
+    x, w, b, gy = rnd((5000, 200), BF, 0), rnd((200,), FF, 1), rnd((200,), FF, 2), rnd((5000, 200), BF, 3)
+    runs = []
+    for _ in range(3):
+        ins = [t.detach().requires_grad_() for t in (x, w, b)]
+        runs.append(torch.autograd.grad(ops.layer_norm(*ins), ins, gy))
+    for r in runs[1:]:
+        for s, t in zip(r, runs[0]):
+            assert torch.equal(s, t)
+
+
+def test_attention_keeps_its_own_mask():
+    """The packed mask is the call's: writing over the tensor before the backward pass changes nothing. A length that was
+    written over is refused, as torch refuses any saved tensor that changed."""
+    q, k, v, go = qkvg(2, 60, 70, 2, 2, 32, BF)
+    mask = (torch.rand(60, 70, generator=torch.Generator().manual_seed(4)) < 0.5).to(DEV)
+    ins = [t.detach().requires_grad_() for t in (q, k, v)]
+    want = torch.autograd.grad(ops.attention(*ins, mask=mask.clone()), ins, go)
+    out = ops.attention(*ins, mask=mask)
+    mask.fill_(False)
+    for a, b in zip(torch.autograd.grad(out, ins, go), want):
+        assert torch.equal(a, b)
+    lengths = torch.tensor([70, 30], dtype=torch.int32, device=DEV)
+    out = ops.attention(*ins, lengths=lengths)
+    lengths.fill_(5)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out, ins, go)
