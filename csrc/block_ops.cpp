@@ -236,7 +236,7 @@ void backward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, con
   if (dk.defined()) p.dk = view(dk);
   if (dv.defined()) p.dv = view(dv);
   const at::Tensor delta = at::empty_like(sv.lse2);
-  attn_bwd_splits(p.B, p.Hkv, p.M, p.Sk, p.causal || p.lengths, p.splits, p.kv_splits);
+  attn_bwd_splits(p.B, p.Hkv, p.M, p.Sk, p.causal != 0, p.splits, p.kv_splits);
   const int64_t dp = (p.D + 31) / 32 * 32, bh = (int64_t)p.B * p.Hkv;
   const int64_t nq = p.splits > 1 ? p.splits * bh * p.M * dp : 0, nk = p.kv_splits > 1 ? 2 * p.kv_splits * bh * p.Sk * dp : 0;
   at::Tensor ws;

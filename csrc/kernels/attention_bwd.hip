@@ -625,12 +625,14 @@ void bwd_d(const AttnParams& p, hipStream_t st) {
 }  // namespace
 
 // Blocks that share a row block's keys (dq) and a key block's rows (dk, dv): as attn_splits, up to two blocks a CU, or
-// four for dk, dv where blocks differ (causal, 2 images, 16 heads that share 2, 8,192 tokens, 128
-// channels: 2,862 / 2,041 / 2,053 us for 512 / 1,024 / 2,048 blocks); at least four tiles each.
-void attn_bwd_splits(int B, int Hkv, int M, int Sk, bool uneven, int& splits, int& kv_splits) {
+// four for causal dk, dv, whose blocks are as unequal as their keys (2 images, 16 heads that share 2, 8,192 tokens, 128
+// channels: 2,862 / 2,041 / 2,053 us for 512 / 1,024 / 2,048 blocks); at least four tiles each. Lengths make blocks empty,
+// not unequal: more than one round of them only costs parts (6 images of 1,531 keys, all full: 122 us for 512, 131 for
+// 1,024; 60 % full: 110 and 106).
+void attn_bwd_splits(int B, int Hkv, int M, int Sk, bool causal, int& splits, int& kv_splits) {
   const int64_t bhn = (int64_t)B * Hkv, qb = (M + 127) / 128 * bhn, kb = std::max<int64_t>(1, (Sk + 127) / 128 * bhn);
   splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / qb, (Sk + 63) / 64 / 4));
-  kv_splits = (int)std::max<int64_t>(1, std::min<int64_t>((uneven ? 1024 : 512) / kb, (M + 63) / 64 / 4));
+  kv_splits = (int)std::max<int64_t>(1, std::min<int64_t>((causal ? 1024 : 512) / kb, (M + 63) / 64 / 4));
 }
 
 int attn_bwd(const AttnParams& p, hipStream_t st) {

@@ -667,7 +667,7 @@ struct AttnMaskArgs {
 int attn_mask_bits(const AttnMaskArgs& a, hipStream_t st);
 int attn_splits(int B, int Hkv, int M, int Sk);      // key splits of a forward call (1: no workspace)
 int attn_fwd(const AttnParams& p, hipStream_t st);
-void attn_bwd_splits(int B, int Hkv, int M, int Sk, bool uneven, int& splits, int& kv_splits);
+void attn_bwd_splits(int B, int Hkv, int M, int Sk, bool causal, int& splits, int& kv_splits);
 int attn_bwd(const AttnParams& p, hipStream_t st);
 
 // ---------------------------------------------------------------- layer_norm.hip
