@@ -365,7 +365,8 @@ template <int TYPE, int V, int LPR, int NV>
 int go(const LayerNormParams& p, bool bwd, bool count, hipStream_t st) {
   constexpr int NT = bwd_threads, RPB = NT / LPR, NTF = LPR > 256 ? LPR : 256, RPBF = NTF / LPR;
   static_assert(LPR <= NT, "a row fits the block");
-  if (count) return (int)std::min<int64_t>(512, (p.rows + RPB - 1) / RPB);
+  // up to four rows a row group: one block, whose sums need no join
+  if (count) return p.rows <= 4 * RPB ? 1 : (int)std::min<int64_t>(512, (p.rows + RPB - 1) / RPB);
   if (bwd)
     ln_bwd_kernel<TYPE, V, LPR, NV, NT><<<p.blocks, NT, 0, st>>>(p);
   else

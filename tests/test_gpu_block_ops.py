@@ -880,3 +880,30 @@ def test_attention_keeps_its_own_mask():
     lengths.fill_(5)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(out, ins, go)
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("D", [32, 64, 80, 128])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_attention_groups_do_not_hear_each_other(bad, D, dt):
+    """Two images packed into one row of tokens: whatever breaks in one - a query, a key, a value, a gradient - leaves
+    the other's output and gradients as they were, bit for bit, and shows in its own."""
+    S, cut = 210, 110                                        # the border inside a tile of rows and of keys
+    group = torch.arange(S, device=DEV) >= cut
+    mask = group[:, None] == group[None]
+    base = qkvg(1, S, S, 2, 1, D, dt)
+
+    def run(ts):
+        q, k, v, go = ts
+        ins = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = ops.attention(*ins, mask=mask)
+        return [out.detach(), *torch.autograd.grad(out, ins, go)]
+
+    want = run(base)
+    for n in range(4):
+        ts = [t.clone() for t in base]
+        ts[n][0, cut - 3, 0, 1] = bad
+        got = run(ts)
+        for a, b in zip(got, want):
+            assert torch.equal(a[:, cut:], b[:, cut:]), n
+        assert not all(torch.isfinite(t[:, :cut]).all() for t in got), n
