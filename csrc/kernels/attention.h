@@ -156,13 +156,30 @@ CFL_DEVICE float finite_sum(const f16v& v) {
   return t;
 }
 
-// eight elements 8s .. 8s + 7 of a result, rounded to 16 bits: the B operand of the second product
-template <class T>
-CFL_DEVICE s8v pack_b(const f16v& v, int s) {
-  const u4v w = {T::pack2(v[8 * s], v[8 * s + 1]), T::pack2(v[8 * s + 2], v[8 * s + 3]),
-                 T::pack2(v[8 * s + 4], v[8 * s + 5]), T::pack2(v[8 * s + 6], v[8 * s + 7])};
-  return __builtin_bit_cast(s8v, w);
-}
+// eight elements 8s .. 8s + 7 of a result, rounded to 16 bits: the B operand of the second product; and (FINE) what
+// that rounding took away, rounded itself: as a second operand it leaves the product with little more than the error
+// of fp32. Twice the second products, so for calls that are not bound by them (attn_fine).
+template <class T, bool FINE>
+struct Packed {
+  s8v hi, lo;
+  CFL_DEVICE void set(const f16v& v, int s) {
+    u4v w, x = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float a = v[8 * s + 2 * j], b = v[8 * s + 2 * j + 1];
+      if (FINE) asm("" : "+v"(a), "+v"(b));                // a product, if it is one, not fused into the difference:
+                                                           // the same bits in both walks
+      w[j] = T::pack2(a, b);
+      if (FINE) x[j] = T::pack2(a - T::lo(w[j]), b - T::hi(w[j]));
+    }
+    hi = __builtin_bit_cast(s8v, w);
+    if (FINE) lo = __builtin_bit_cast(s8v, x);
+  }
+  CFL_DEVICE f16v mma(const s8v& a, f16v c) const {
+    c = T::mma(a, hi, c);
+    return FINE ? T::mma(a, lo, c) : c;
+  }
+};
 
 // 32 channels 32 * dt .. + 31 of one token row per lane pair (c, c + 32): four quads each, exchanged between the
 // halves so that a lane stores 16 contiguous bytes (lane half h: channels 16s + 8h .. + 7). rest: if given, what the

@@ -33,7 +33,7 @@ constexpr float SLACK = 8.f;
 constexpr int FEW_ROWS = 32;
 
 // QT: 32-row tiles per wave; WR x WK: waves along the rows and along the keys of a tile; KW keys per wave and tile
-template <class T, int DP, int QT, int WR, int WK, int KW, int MINW, int KIND>
+template <class T, int DP, int QT, int WR, int WK, int KW, int MINW, int KIND, bool FINE>
 __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const AttnParams p) {
   constexpr int NT = 64 * WR * WK, KT = KW * WK, TILE = KT * DP, CPR = DP / 8, CH = KT * CPR / NT;
   constexpr int NK = KW / 32, NKK = DP / 16, ND = DP / 32;
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
             }
         }
         __builtin_amdgcn_s_setprio(0);
-        s8v pb[QT][2 * NK];
+        Packed<T, FINE> pb[QT][2 * NK];
 #pragma unroll
         for (int u = 0; u < QT; ++u) {
           float mx = s[0][u][0];
@@ -243,8 +243,8 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
               s[k][u][e] = exp2_(fmaf(s[k][u][e], sc, -ms));
               sum += s[k][u][e];
             }
-            pb[u][2 * k] = pack_b<T>(s[k][u], 0);
-            pb[u][2 * k + 1] = pack_b<T>(s[k][u], 1);
+            pb[u][2 * k].set(s[k][u], 0);
+            pb[u][2 * k + 1].set(s[k][u], 1);
           }
           l[u] += sum;
         }
@@ -259,10 +259,10 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
               __builtin_amdgcn_sched_barrier(0);           // few registers matter here, not speed
               a = clean<T>(a, pos, neg);
 #pragma unroll
-              for (int u = 0; u < QT; ++u) poison<T>(acc[d][u], pos, neg, pb[u][ks]);
+              for (int u = 0; u < QT; ++u) poison<T>(acc[d][u], pos, neg, pb[u][ks].hi);
             }
 #pragma unroll
-            for (int u = 0; u < QT; ++u) acc[d][u] = T::mma(a, pb[u][ks], acc[d][u]);
+            for (int u = 0; u < QT; ++u) acc[d][u] = pb[u][ks].mma(a, acc[d][u]);
           }
       }
       __builtin_amdgcn_s_setprio(0);
@@ -438,21 +438,22 @@ __global__ __launch_bounds__(256) void attn_mask_kernel(const AttnMaskArgs a) {
   if (lane == 0) a.cls[unit] = any == 0 ? 0 : all == ~0ull ? 2 : 1;
 }
 
-template <class T, int DP, int QT, int WR, int WK, int KW, int MINW>
+template <class T, int DP, int QT, int WR, int WK, int KW, int MINW, bool FINE>
 void launch(const AttnParams& p, hipStream_t st) {
   const int64_t n = (int64_t)((p.M + 32 * QT * WR - 1) / (32 * QT * WR)) * p.B * p.Hkv * p.splits;
   if (p.mask.bits)
-    attn_fwd_kernel<T, DP, QT, WR, WK, KW, MINW, ATTN_MASK><<<(unsigned)n, 64 * WR * WK, 0, st>>>(p);
+    attn_fwd_kernel<T, DP, QT, WR, WK, KW, MINW, ATTN_MASK, FINE><<<(unsigned)n, 64 * WR * WK, 0, st>>>(p);
   else if (p.causal)
-    attn_fwd_kernel<T, DP, QT, WR, WK, KW, MINW, ATTN_CAUSAL><<<(unsigned)n, 64 * WR * WK, 0, st>>>(p);
+    attn_fwd_kernel<T, DP, QT, WR, WK, KW, MINW, ATTN_CAUSAL, FINE><<<(unsigned)n, 64 * WR * WK, 0, st>>>(p);
   else
-    attn_fwd_kernel<T, DP, QT, WR, WK, KW, MINW, ATTN_PLAIN><<<(unsigned)n, 64 * WR * WK, 0, st>>>(p);
+    attn_fwd_kernel<T, DP, QT, WR, WK, KW, MINW, ATTN_PLAIN, FINE><<<(unsigned)n, 64 * WR * WK, 0, st>>>(p);
 }
 
 template <class T, int DP>
 void fwd(const AttnParams& p, hipStream_t st) {
-  if (p.M <= FEW_ROWS) launch<T, DP, 1, 1, 4, 32, 1>(p, st);
-  else launch<T, DP, 1, 4, 1, 64, 2>(p, st);
+  if (p.M <= FEW_ROWS) launch<T, DP, 1, 1, 4, 32, 1, true>(p, st);       // bound by memory
+  else if (attn_fine(p)) launch<T, DP, 1, 4, 1, 64, 2, true>(p, st);
+  else launch<T, DP, 1, 4, 1, 64, 2, false>(p, st);
   if (p.splits > 1) {
     const int64_t n = (int64_t)p.B * p.Hkv * p.M * (DP / 4);
     attn_join_kernel<T, DP><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(p);
@@ -475,6 +476,18 @@ int attn_mask_bits(const AttnMaskArgs& a, hipStream_t st) {
   if ((units + 3) / 4 > 0x7fffffff) return 1;
   attn_mask_kernel<<<(unsigned)((units + 3) / 4), 256, 0, st>>>(a);
   return hipGetLastError() == hipSuccess ? 0 : 3;
+}
+
+// Calls of up to 2^24 pairs of a query and a key keep P and dS in two 16-bit parts (attention.h Packed). With few keys
+// or rows the rounding to one part does not average out: over 80 calls drawn from 1 to 700 tokens the error of dq is
+// 1.44 times that of 16-bit products with fp32 softmax on average and 1.5 to 1.8 in six of them, against 1.03 and none
+// with two parts; dv 1.02 against 0.79. The price (us, one part -> two): 16 images x 8 heads x 256 tokens of 32 channels
+// forward 6.9 -> 7.7, dq 8.9 -> 10.1, dk and dv 8.1 -> 10.3, less than the launches around them; at the bound, 16 x 8 x
+// 360 tokens of 64 channels, 18.0 -> 21.0, 19.6 -> 22.1, 18.8 -> 24.6. Larger calls are bound by the matrix
+// instructions and keep one part: 16 x 8 x 1,024 tokens of 64 channels 50 against 66, and 161 against 202 backward.
+bool attn_fine(const AttnParams& p) {
+  const int t = cfl_tune(TUNE_ATTN_FINE);
+  return t ? t == 2 : (double)p.B * p.Hkv * p.M * p.Sk <= 16777216.0;
 }
 
 // Blocks that share the keys of a row block: enough for two blocks a CU where there are few row blocks, at least four

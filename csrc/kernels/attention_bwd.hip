@@ -22,7 +22,7 @@ namespace {
 using namespace attn;
 
 // dq: QT 32-row tiles per wave, 4 waves along the rows, tiles of KT keys
-template <class T, int DP, int QT, int KIND>
+template <class T, int DP, int QT, int KIND, bool FINE>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
   constexpr int NT = 256, KT = 64, TILE = KT * DP, CPR = DP / 8, CH = KT * CPR / NT;
   static_assert(KT * CPR % NT == 0, "whole DMA instructions");
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
 #pragma unroll
             for (int u = 0; u < QT; ++u) dp[u] = T::mma(a, gf[u][kk], dp[u]);
           }
-          s8v db[QT][2];
+          Packed<T, FINE> db[QT][2];
           if (DP == 128) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int u = 0; u < QT; ++u) {
@@ -223,8 +223,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
               const float ds = s[u][e] * dp[u][e];
               s[u][e] = SAFE && s[u][e] == 0.f ? 0.f : ds;
             }
-            db[u][0] = pack_b<T>(s[u], 0);
-            db[u][1] = pack_b<T>(s[u], 1);
+            db[u][0].set(s[u], 0);
+            db[u][1].set(s[u], 1);
           }
           if (DP == 128) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
                 a = clean<T>(a, pos, neg);
               }
 #pragma unroll
-              for (int u = 0; u < QT; ++u) acc[d][u] = T::mma(a, db[u][ks], acc[d][u]);
+              for (int u = 0; u < QT; ++u) acc[d][u] = db[u][ks].mma(a, acc[d][u]);
             }
         }
       }
@@ -280,7 +280,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
 // dk, dv: KQ 32-key tiles per wave, 4 waves along the keys, tiles of RT rows. The wave's keys are B operands in registers
 // for the whole walk, its values too, or (VL: from 96 channels, where dk and dv take half of the 256 registers that let
 // two waves share a SIMD) in LDS.
-template <class T, int DP, int KQ, int RT, bool VL, int KIND>
+template <class T, int DP, int KQ, int RT, bool VL, int KIND, bool FINE>
 __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
   constexpr int NT = 256, TILE = RT * DP, CPR = DP / 8, CH = RT * CPR / NT, VTILE = VL ? 128 * KQ * DP : 0;
   static_assert(RT * CPR % NT == 0 && VTILE / 8 % NT == 0, "whole DMA instructions");
@@ -466,7 +466,9 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
             dp[u] = T::mma(a, VL ? frag_x<DP>(svals + 32 * u * DP, fo, kk) : vf[u][VL ? 0 : kk], dp[u]);
           if (VL && kk % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         }
-        s8v pb[KQ][2], db[KQ][2];
+        // at 128 channels the second part of P does not fit into the registers beside the conditions
+        Packed<T, FINE && (DP < 128 || KIND == ATTN_PLAIN)> pb[KQ][2];
+        Packed<T, FINE> db[KQ][2];
         if (VL) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int u = 0; u < KQ; ++u) {
@@ -490,15 +492,15 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[u][e] = (e & 3) + 8 * (e >> 2) >= from ? s[u][e] : 0.f;
           }
-          pb[u][0] = pack_b<T>(s[u], 0);
-          pb[u][1] = pack_b<T>(s[u], 1);
+          pb[u][0].set(s[u], 0);
+          pb[u][1].set(s[u], 1);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             dp[u][e] *= s[u][e];
             if constexpr (SAFE) dp[u][e] = s[u][e] == 0.f ? 0.f : dp[u][e];
           }
-          db[u][0] = pack_b<T>(dp[u], 0);
-          db[u][1] = pack_b<T>(dp[u], 1);
+          db[u][0].set(dp[u], 0);
+          db[u][1].set(dp[u], 1);
         }
         if (VL) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -511,10 +513,10 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
               __builtin_amdgcn_sched_barrier(0);           // few registers matter here, not speed
               a = clean<T>(a, pos, neg);
 #pragma unroll
-              for (int u = 0; u < KQ; ++u) poison<T>(dv[d][u], pos, neg, pb[u][ks]);
+              for (int u = 0; u < KQ; ++u) poison<T>(dv[d][u], pos, neg, pb[u][ks].hi);
             }
 #pragma unroll
-            for (int u = 0; u < KQ; ++u) dv[d][u] = T::mma(a, pb[u][ks], dv[d][u]);
+            for (int u = 0; u < KQ; ++u) dv[d][u] = pb[u][ks].mma(a, dv[d][u]);
           }
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
@@ -527,7 +529,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
               a = clean<T>(a, pos, neg);
             }
 #pragma unroll
-            for (int u = 0; u < KQ; ++u) dk[d][u] = T::mma(a, db[u][ks], dk[d][u]);
+            for (int u = 0; u < KQ; ++u) dk[d][u] = db[u][ks].mma(a, dk[d][u]);
           }
       }
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -592,15 +594,15 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(const float* ws, int spli
   *reinterpret_cast<uint2*>(o) = make_uint2(T::pack2(a.x, a.y), T::pack2(a.z, a.w));
 }
 
-template <class T, int DP, int KIND>
+template <class T, int DP, int KIND, bool FINE>
 void bwd(const AttnParams& p, hipStream_t st) {
   const int64_t bhn = (int64_t)p.B * p.Hkv;
-  attn_dq_kernel<T, DP, 1, KIND><<<(unsigned)((p.M + 127) / 128 * bhn * p.splits), 256, 0, st>>>(p);
+  attn_dq_kernel<T, DP, 1, KIND, FINE><<<(unsigned)((p.M + 127) / 128 * bhn * p.splits), 256, 0, st>>>(p);
   if (p.splits > 1 && p.dq.p)
     attn_sum_kernel<T, DP><<<(unsigned)((bhn * p.M * (DP / 4) + 255) / 256), 256, 0, st>>>(
         p.ws_o, p.splits, p.dq, p.B, p.Hkv, p.G, p.M, p.D, p.div_g, nullptr);
   if ((p.dk.p == nullptr && p.dv.p == nullptr) || p.Sk == 0) return;
-  attn_dkv_kernel<T, DP, 1, DP == 128 ? 32 : 64, DP >= 96, KIND>
+  attn_dkv_kernel<T, DP, 1, DP == 128 ? 32 : 64, DP >= 96, KIND, FINE>
       <<<(unsigned)((p.Sk + 127) / 128 * bhn * p.kv_splits), 256, 0, st>>>(p);
   if (p.kv_splits > 1) {
     const int64_t n = bhn * p.Sk;
@@ -616,10 +618,10 @@ void bwd(const AttnParams& p, hipStream_t st) {
 
 template <class T, int KIND>
 void bwd_d(const AttnParams& p, hipStream_t st) {
-  if (p.D <= 32) bwd<T, 32, KIND>(p, st);
-  else if (p.D <= 64) bwd<T, 64, KIND>(p, st);
-  else if (p.D <= 96) bwd<T, 96, KIND>(p, st);
-  else bwd<T, 128, KIND>(p, st);
+  if (p.D <= 32) attn_fine(p) ? bwd<T, 32, KIND, true>(p, st) : bwd<T, 32, KIND, false>(p, st);
+  else if (p.D <= 64) attn_fine(p) ? bwd<T, 64, KIND, true>(p, st) : bwd<T, 64, KIND, false>(p, st);
+  else if (p.D <= 96) attn_fine(p) ? bwd<T, 96, KIND, true>(p, st) : bwd<T, 96, KIND, false>(p, st);
+  else attn_fine(p) ? bwd<T, 128, KIND, true>(p, st) : bwd<T, 128, KIND, false>(p, st);
 }
 
 }  // namespace

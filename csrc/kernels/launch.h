@@ -552,7 +552,8 @@ enum TuneKey {
   TUNE_PWB = 56,               // encoder pointwise backward: 0 = fused dgrad + wgrad (pw_bwd.hip), 1 = pw.hip dgrad +
                                //   deferred wgrad (round 5)
   TUNE_WGRAD_REPS = 57,         // generic weight-gradient replica rows (conv_wgrad_slabs; default WGRAD_REPLICAS)
-  TUNE_N = 58
+  TUNE_ATTN_FINE = 58,         // attention: P and dS in two 16-bit parts; 0 = small calls (attn_fine), 1 = never, 2 = always
+  TUNE_N = 59
 };
 int cfl_tune(int key);
 void cfl_set_tune(int key, int value);
@@ -665,6 +666,7 @@ struct AttnMaskArgs {
 };
 
 int attn_mask_bits(const AttnMaskArgs& a, hipStream_t st);
+bool attn_fine(const AttnParams& p);                 // P and dS in two 16-bit parts
 int attn_splits(int B, int Hkv, int M, int Sk);      // key splits of a forward call (1: no workspace)
 int attn_fwd(const AttnParams& p, hipStream_t st);
 void attn_bwd_splits(int B, int Hkv, int M, int Sk, bool causal, int& splits, int& kv_splits);
