@@ -466,9 +466,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
             dp[u] = T::mma(a, VL ? frag_x<DP>(svals + 32 * u * DP, fo, kk) : vf[u][VL ? 0 : kk], dp[u]);
           if (VL && kk % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         }
-        // at 128 channels the second part of P does not fit into the registers beside the conditions
-        Packed<T, FINE && (DP < 128 || KIND == ATTN_PLAIN)> pb[KQ][2];
-        Packed<T, FINE> db[KQ][2];
+        Packed<T, FINE> pb[KQ][2], db[KQ][2];
         if (VL) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int u = 0; u < KQ; ++u) {
@@ -503,34 +501,41 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
           db[u][1].set(dp[u], 1);
         }
         if (VL) __builtin_amdgcn_sched_barrier(0);
+        auto add_dv = [&]() {
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
+          for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-          for (int d = 0; d < ND; ++d) {
-            s8v a = frag_t<DP>(sg + (32 * n + 16 * ks) * DP, ta, d);
-            if constexpr (SAFE) {
-              s8v pos, neg;
-              __builtin_amdgcn_sched_barrier(0);           // few registers matter here, not speed
-              a = clean<T>(a, pos, neg);
+            for (int d = 0; d < ND; ++d) {
+              s8v a = frag_t<DP>(sg + (32 * n + 16 * ks) * DP, ta, d);
+              if constexpr (SAFE) {
+                s8v pos, neg;
+                __builtin_amdgcn_sched_barrier(0);           // few registers matter here, not speed
+                a = clean<T>(a, pos, neg);
 #pragma unroll
-              for (int u = 0; u < KQ; ++u) poison<T>(dv[d][u], pos, neg, pb[u][ks].hi);
+                for (int u = 0; u < KQ; ++u) poison<T>(dv[d][u], pos, neg, pb[u][ks].hi);
+              }
+#pragma unroll
+              for (int u = 0; u < KQ; ++u) dv[d][u] = pb[u][ks].mma(a, dv[d][u]);
             }
+        };
+        auto add_dk = [&]() {
 #pragma unroll
-            for (int u = 0; u < KQ; ++u) dv[d][u] = pb[u][ks].mma(a, dv[d][u]);
-          }
+          for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
+            for (int d = 0; d < ND; ++d) {
+              s8v a = frag_t<DP>(sq + (32 * n + 16 * ks) * DP, ta, d);
+              if constexpr (SAFE) {                            // an allowed query that is not finite shows in its scores
+                s8v pos, neg;
+                __builtin_amdgcn_sched_barrier(0);           // few registers matter here, not speed
+                a = clean<T>(a, pos, neg);
+              }
 #pragma unroll
-          for (int d = 0; d < ND; ++d) {
-            s8v a = frag_t<DP>(sq + (32 * n + 16 * ks) * DP, ta, d);
-            if constexpr (SAFE) {                            // an allowed query that is not finite shows in its scores
-              s8v pos, neg;
-              __builtin_amdgcn_sched_barrier(0);           // few registers matter here, not speed
-              a = clean<T>(a, pos, neg);
+              for (int u = 0; u < KQ; ++u) dk[d][u] = db[u][ks].mma(a, dk[d][u]);
             }
-#pragma unroll
-            for (int u = 0; u < KQ; ++u) dk[d][u] = db[u][ks].mma(a, dk[d][u]);
-          }
+        };
+        if (!SAFE) add_dv();                                 // clean and poison need the registers of db
+        add_dk();
+        if (SAFE) add_dv();
       }
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
