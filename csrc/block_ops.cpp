@@ -24,9 +24,15 @@ using torch::autograd::variable_list;
 
 hipStream_t stream() { return c10::hip::getCurrentHIPStream().stream(); }
 
-void ok(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed (code ", rc, ")"); }
+void ok(int rc, const char* what) {
+  TORCH_CHECK(rc != 2, what, ": too large for one launch");
+  TORCH_CHECK(rc == 0, what, " failed (code ", rc, ")");
+}
 
+// also for a tangent of forward-mode derivatives: the autograd function refuses it, the plain call would drop it
 bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
+  for (const at::Tensor* t : ts)
+    if (t->defined() && t->_fw_grad(0).defined()) return true;
   if (!at::GradMode::is_enabled()) return false;
   for (const at::Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;
@@ -595,6 +601,8 @@ at::Tensor rotary(const at::Tensor& x, const at::Tensor& pos, const std::vector<
                          pos.size(2) == S),
                     "rotary: positions must be (", A, ", ", S, ") or (", A, ", ", B, ", ", S, "), got ", pos.sizes());
   TORCH_CHECK_VALUE(!pos.requires_grad(), "rotary: positions have no gradient");
+  constexpr int64_t top = (int64_t)1 << 31;
+  TORCH_CHECK_VALUE(B < top && S < top && x.size(2) < top && x.size(3) < top, "rotary: too large: x ", x.sizes());
   TORCH_CHECK(x.is_cuda(), "rotary: x must be a device tensor");
   check_device(pos, x, "rotary: positions");
   pl.theta = theta;

@@ -473,15 +473,15 @@ void fwd_d(const AttnParams& p, hipStream_t st) {
 int attn_mask_bits(const AttnMaskArgs& a, hipStream_t st) {
   const int64_t units = (int64_t)a.Bm * a.Hm * ((a.Im + 31) / 32) * a.words;
   if (units == 0) return 0;
-  if ((units + 3) / 4 > 0x7fffffff) return 1;
+  if ((units + 3) / 4 > ATTN_MAX_BLOCKS) return 2;
   attn_mask_kernel<<<(unsigned)((units + 3) / 4), 256, 0, st>>>(a);
   return hipGetLastError() == hipSuccess ? 0 : 3;
 }
 
 // Calls of up to 2^24 pairs of a query and a key keep P and dS in two 16-bit parts (attention.h Packed). With few keys
-// or rows the rounding to one part does not average out: over 80 calls drawn from 1 to 700 tokens the error of dq is
-// 1.44 times that of 16-bit products with fp32 softmax on average and 1.5 to 1.8 in six of them, against 1.03 and none
-// with two parts; dv 1.02 against 0.79. The price (us, one part -> two): 16 images x 8 heads x 256 tokens of 32 channels
+// or rows the rounding to one part does not average out: over 80 calls of mixed sizes the error of dq is 1.44 times that
+// of rounding only the results on average and more than 1.5 times in five of them, against 1.03 and none with two parts;
+// dv 1.02 against 0.79. The price (us, one part -> two): 16 images x 8 heads x 256 tokens of 32 channels
 // forward 6.9 -> 7.7, dq 8.9 -> 10.1, dk and dv 8.1 -> 10.3, less than the launches around them; at the bound, 16 x 8 x
 // 360 tokens of 64 channels, 18.0 -> 21.0, 19.6 -> 22.1, 18.8 -> 24.6. Larger calls are bound by the matrix
 // instructions and keep one part: 16 x 8 x 1,024 tokens of 64 channels 50 against 66, and 161 against 202 backward.
@@ -501,8 +501,9 @@ int attn_splits(int B, int Hkv, int M, int Sk) {
 
 int attn_fwd(const AttnParams& p, hipStream_t st) {
   if (p.D < 8 || p.D > 128 || p.D % 8 || p.M < 1 || p.Sk < 0 || p.splits < 1) return 1;
-  const int64_t grid = ((int64_t)p.M + 31) / 32 * p.B * p.Hkv * p.splits;
-  if (grid > 0x7fffffff) return 2;
+  const int rows = p.M <= FEW_ROWS ? FEW_ROWS : 128;
+  const int64_t grid = ((int64_t)p.M + rows - 1) / rows * p.B * p.Hkv * p.splits;
+  if (grid > ATTN_MAX_BLOCKS) return 2;
   if (p.fp16) fwd_d<FP16>(p, st);
   else fwd_d<BF16>(p, st);
   return hipGetLastError() == hipSuccess ? 0 : 3;

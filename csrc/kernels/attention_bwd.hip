@@ -644,8 +644,8 @@ void attn_bwd_splits(int B, int Hkv, int M, int Sk, bool causal, int& splits, in
 
 int attn_bwd(const AttnParams& p, hipStream_t st) {
   if (p.D < 8 || p.D > 128 || p.D % 8 || p.M < 1 || p.Sk < 0 || p.splits < 1 || p.kv_splits < 1) return 1;
-  if ((p.M + 127) / 128 * (int64_t)p.B * p.Hkv * p.splits > 0x7fffffff ||
-      (p.Sk + 127) / 128 * (int64_t)p.B * p.Hkv * p.kv_splits > 0x7fffffff)
+  if ((p.M + 127) / 128 * (int64_t)p.B * p.Hkv * p.splits > ATTN_MAX_BLOCKS ||
+      (p.Sk + 127) / 128 * (int64_t)p.B * p.Hkv * p.kv_splits > ATTN_MAX_BLOCKS)
     return 2;
   const int kind = p.mask.bits ? ATTN_MASK : p.causal ? ATTN_CAUSAL : ATTN_PLAIN;
   if (kind == ATTN_MASK) p.fp16 ? bwd_d<FP16, ATTN_MASK>(p, st) : bwd_d<BF16, ATTN_MASK>(p, st);

@@ -666,6 +666,7 @@ struct AttnMaskArgs {
 };
 
 int attn_mask_bits(const AttnMaskArgs& a, hipStream_t st);
+constexpr int64_t ATTN_MAX_BLOCKS = 0xffffff;        // of 256 threads: a launch has fewer than 2^32
 bool attn_fine(const AttnParams& p);                 // P and dS in two 16-bit parts
 int attn_splits(int B, int Hkv, int M, int Sk);      // key splits of a forward call (1: no workspace)
 int attn_fwd(const AttnParams& p, hipStream_t st);

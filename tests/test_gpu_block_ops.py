@@ -907,3 +907,24 @@ def test_attention_groups_do_not_hear_each_other(bad, D, dt):
         for a, b in zip(got, want):
             assert torch.equal(a[:, cut:], b[:, cut:]), n
         assert not all(torch.isfinite(t[:, :cut]).all() for t in got), n
+
+
+def test_attention_refuses_more_blocks_than_a_launch_has():
+    q = torch.zeros(1 << 24, 1, 1, 8, dtype=BF, device=DEV)
+    with pytest.raises(RuntimeError, match="too large for one launch"):
+        ops.attention(q, q, q)
+    assert not ops.attention(q[1:], q[1:], q[1:]).any()
+
+
+def test_forward_mode_tangents_are_refused():
+    """No forward-mode derivative: the call says so instead of dropping the tangent."""
+    import torch.autograd.forward_ad as fwd
+    q, k, v, go = qkvg(1, 4, 4, 1, 1, 32, BF)
+    pos = torch.arange(4, device=DEV)[None]
+    with fwd.dual_level():
+        d = fwd.make_dual(q, go)
+        for call in (lambda: ops.attention(d, k, v), lambda: ops.layer_norm(d), lambda: ops.rotary(d, pos, (32,))):
+            with pytest.raises(RuntimeError):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError):
+                call()
