@@ -255,7 +255,8 @@ __global__ __launch_bounds__(NT) void ln_bwd_kernel(const LayerNormParams p) {
     load_row<TYPE, V, NV>(xb + (r + step) * p.x_stride, col, p.C, r + step < p.rows, xn);
     load_row<TYPE, V, NV>(gb + (r + step) * p.gy_stride, col, p.C, r + step < p.rows, gn);
     float d[NV];
-    const float rs = center<LPR, NV, V>(x, col, p.C, p.eps, sh, red[par][gr], d);
+    float rs = center<LPR, NV, V>(x, col, p.C, p.eps, sh, red[par][gr], d);
+    rs = ok ? rs : 0.f;                                    // no row: 1 / sqrt(eps) may be infinite, and 0 times it NaN
     float s0 = 0.f, s1 = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; ++k)

@@ -408,6 +408,12 @@ def test_layer_norm_large_mean_and_constant_rows():
             assert float(dx.abs().max()) <= tol
 
 
+@pytest.mark.parametrize("rows,C", [(3, 32), (70, 33), (130, 256), (1, 1000), (5, 4096), (700, 64)])
+def test_layer_norm_without_epsilon(rows, C):
+    """eps = 0: no part of the card that holds no row may add to the weights' gradients (0 / 0)."""
+    check_norm(rnd((rows, C), BF, 1), rnd((C,), FF, 2), rnd((C,), FF, 3), rnd((rows, C), BF, 4), eps=0.0)
+
+
 def test_layer_norm_frozen_inputs_and_empty_rows():
     x, w, b = rnd((50, 64), BF, 0), rnd((64,), FF, 1), rnd((64,), FF, 2)
     gy = rnd((50, 64), BF, 3)
