@@ -89,7 +89,8 @@ Shape check_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor
   constexpr int64_t top = (int64_t)1 << 30;
   TORCH_CHECK_VALUE(s.Sq * (s.Hq / s.Hkv) < top && s.Sk < top && s.B * s.Hkv < top && s.Hq * s.D < ((int64_t)1 << 23),
                     "attention: too large: q ", q.sizes(), ", k ", k.sizes());
-  TORCH_CHECK_VALUE(std::isfinite(scale) && scale > 0, "attention: scale must be positive and finite, got ", scale);
+  TORCH_CHECK_VALUE((float)scale > 0 && std::isfinite(2 * (float)scale),    // the kernels take it times log2(e)
+                    "attention: scale must be positive and finite in float32, got ", scale);
   if (mask) {
     TORCH_CHECK_TYPE(mask->scalar_type() == at::kBool, "attention: mask must be bool (True: may attend), is ",
                      mask->scalar_type());

@@ -97,3 +97,9 @@ def test_self_attention2d_refuses(kw):
             "w_qkv": torch.zeros(1, 1, 64, 12 * 32), "w_out": torch.zeros(1, 1, 128, 64), "heads": 4}
     with pytest.raises(ValueError):
         ops.self_attention2d(**{**base, **kw})
+
+
+@pytest.mark.parametrize("scale", [1e-50, 3e38, 1e39, math.inf])
+def test_attention_refuses_scales_outside_float32(scale):
+    with pytest.raises(ValueError, match="float32"):
+        ops.attention(Q, KV, KV, scale=scale)
