@@ -158,7 +158,7 @@ CFL_DEVICE float finite_sum(const f16v& v) {
 
 // eight elements 8s .. 8s + 7 of a result, rounded to 16 bits: the B operand of the second product; and (FINE) what
 // that rounding took away, rounded itself: as a second operand it leaves the product with little more than the error
-// of fp32. Twice the second products, so for calls that are not bound by them (attn_fine).
+// of fp32, for twice the second products (attn_fine).
 template <class T, bool FINE>
 struct Packed {
   s8v hi, lo;

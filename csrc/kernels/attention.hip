@@ -5,8 +5,8 @@
 // the lane 32 away, the rescaling factor is the lane's own scalar, and exp(S^T) rounded to 16 bits is the B operand of
 // O^T = V^T P^T as it stands. K and V tiles go from memory to LDS by LDS-DMA loads, one tile ahead.
 //
-// Rounding: scores, maximum, sum and output accumulate in fp32. P is rounded to the inputs' type (relative error at most
-// half a step per term, independent from key to key), the output once.
+// Rounding: scores, maximum, sum and output accumulate in fp32. P enters the second product in two parts of the inputs'
+// type (attn_fine), the output is rounded once.
 // Split. Four waves own 32 rows each and share the tiles (64 keys); up to 32 rows in all, the waves split a tile's keys
 // instead and join through LDS. Few row blocks: blocks share a walk (attn_splits) and a second launch joins the parts.
 // 256 registers, two waves a SIMD or more: at 512 the compiler puts the first product's result into accumulation
@@ -452,7 +452,7 @@ void launch(const AttnParams& p, hipStream_t st) {
 template <class T, int DP>
 void fwd(const AttnParams& p, hipStream_t st) {
   if (p.M <= FEW_ROWS) launch<T, DP, 1, 1, 4, 32, 1, true>(p, st);       // bound by memory
-  else if (attn_fine(p)) launch<T, DP, 1, 4, 1, 64, 2, true>(p, st);
+  else if (attn_fine()) launch<T, DP, 1, 4, 1, 64, 2, true>(p, st);
   else launch<T, DP, 1, 4, 1, 64, 2, false>(p, st);
   if (p.splits > 1) {
     const int64_t n = (int64_t)p.B * p.Hkv * p.M * (DP / 4);
@@ -478,17 +478,13 @@ int attn_mask_bits(const AttnMaskArgs& a, hipStream_t st) {
   return hipGetLastError() == hipSuccess ? 0 : 3;
 }
 
-// Calls of up to 2^24 pairs of a query and a key keep P and dS in two 16-bit parts (attention.h Packed). With few keys
-// or rows the rounding to one part does not average out: over 80 calls of mixed sizes the error of dq is 1.44 times that
-// of rounding only the results on average and more than 1.5 times in five of them, against 1.03 and none with two parts;
-// dv 1.02 against 0.79. The price (us, one part -> two): 16 images x 8 heads x 256 tokens of 32 channels
-// forward 6.9 -> 7.7, dq 8.9 -> 10.1, dk and dv 8.1 -> 10.3, less than the launches around them; at the bound, 16 x 8 x
-// 360 tokens of 64 channels, 18.0 -> 21.0, 19.6 -> 22.1, 18.8 -> 24.6. Larger calls are bound by the matrix
-// instructions and keep one part: 16 x 8 x 1,024 tokens of 64 channels 50 against 66, and 161 against 202 backward.
-bool attn_fine(const AttnParams& p) {
-  const int t = cfl_tune(TUNE_ATTN_FINE);
-  return t ? t == 2 : (double)p.B * p.Hkv * p.M * p.Sk <= 16777216.0;
-}
+// P and dS are operands of 16 bits in the second products. Rounded to one part they cost as much as the rounding of the
+// results does: the errors of dq, dk, dv and the output are 1.37 to 1.48 times those of rounding nothing but the results.
+// With what that rounding took away as a second operand (attention.h Packed) they are 1.00 to 1.02, at any size of call,
+// so two parts are the rule and one part is the tuning key's. The price is a second set of second products (us, one
+// part -> two, forward and backward): 16 images x 8 heads x 1,024 tokens of 64 channels 48 -> 63 and 144 -> 189, 2 x 16
+// heads x 4,096 tokens of 128 channels 278 -> 372 and 874 -> 1,128.
+bool attn_fine() { return cfl_tune(TUNE_ATTN_FINE) != 1; }
 
 // Blocks that share the keys of a row block: enough for two blocks a CU where there are few row blocks, at least four
 // tiles each. (Blocks of 64 rows with two waves along the keys instead, for such grids, were slower: 4 images x 8 heads

@@ -11,8 +11,8 @@
 // leave one wave a SIMD: slower at every width but 32 (128 channels 1,045 us against 953 then).
 // delta is taken from the output before its rounding (o + what that took away): with few keys dp - delta cancels, and a
 // rounded o would leave its whole step there.
-// Rounding: P and dS are rounded to the inputs' type as operands of the second products; everything else is fp32 until
-// the gradients are rounded once.
+// Rounding: P and dS enter the second products in two parts of the inputs' type (attn_fine); everything else is fp32
+// until the gradients are rounded once.
 #include <algorithm>
 
 #include "attention.h"
@@ -623,10 +623,10 @@ void bwd(const AttnParams& p, hipStream_t st) {
 
 template <class T, int KIND>
 void bwd_d(const AttnParams& p, hipStream_t st) {
-  if (p.D <= 32) attn_fine(p) ? bwd<T, 32, KIND, true>(p, st) : bwd<T, 32, KIND, false>(p, st);
-  else if (p.D <= 64) attn_fine(p) ? bwd<T, 64, KIND, true>(p, st) : bwd<T, 64, KIND, false>(p, st);
-  else if (p.D <= 96) attn_fine(p) ? bwd<T, 96, KIND, true>(p, st) : bwd<T, 96, KIND, false>(p, st);
-  else attn_fine(p) ? bwd<T, 128, KIND, true>(p, st) : bwd<T, 128, KIND, false>(p, st);
+  if (p.D <= 32) attn_fine() ? bwd<T, 32, KIND, true>(p, st) : bwd<T, 32, KIND, false>(p, st);
+  else if (p.D <= 64) attn_fine() ? bwd<T, 64, KIND, true>(p, st) : bwd<T, 64, KIND, false>(p, st);
+  else if (p.D <= 96) attn_fine() ? bwd<T, 96, KIND, true>(p, st) : bwd<T, 96, KIND, false>(p, st);
+  else attn_fine() ? bwd<T, 128, KIND, true>(p, st) : bwd<T, 128, KIND, false>(p, st);
 }
 
 }  // namespace

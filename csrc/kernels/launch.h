@@ -552,7 +552,7 @@ enum TuneKey {
   TUNE_PWB = 56,               // encoder pointwise backward: 0 = fused dgrad + wgrad (pw_bwd.hip), 1 = pw.hip dgrad +
                                //   deferred wgrad (round 5)
   TUNE_WGRAD_REPS = 57,         // generic weight-gradient replica rows (conv_wgrad_slabs; default WGRAD_REPLICAS)
-  TUNE_ATTN_FINE = 58,         // attention: P and dS in two 16-bit parts; 0 = small calls (attn_fine), 1 = never, 2 = always
+  TUNE_ATTN_FINE = 58,         // attention: P and dS in two 16-bit parts; 0 = always, 1 = in one part (attn_fine), 2 = as 0
   TUNE_N = 59
 };
 int cfl_tune(int key);
@@ -667,7 +667,7 @@ struct AttnMaskArgs {
 
 int attn_mask_bits(const AttnMaskArgs& a, hipStream_t st);
 constexpr int64_t ATTN_MAX_BLOCKS = 0xffffff;        // of 256 threads: a launch has fewer than 2^32
-bool attn_fine(const AttnParams& p);                 // P and dS in two 16-bit parts
+bool attn_fine();                                    // P and dS in two 16-bit parts
 int attn_splits(int B, int Hkv, int M, int Sk);      // key splits of a forward call (1: no workspace)
 int attn_fwd(const AttnParams& p, hipStream_t st);
 void attn_bwd_splits(int B, int Hkv, int M, int Sk, bool causal, int& splits, int& kv_splits);

@@ -1,0 +1,101 @@
+"""How near attention comes to rounding nothing but its results, whatever the call's size and the magnitude of its
+values (marked gpu).
+
+The measure is the 2-norm of an output's error over that of the 64-bit result rounded to the tensors' type. 1 is an
+output whose only error is its own rounding. What two 16-bit parts of a weight leave is below 2^-7 of one part's
+rounding, fp32 scores and sums of these sizes are off by less than 2^-17 relative, a tenth of that at most: LIMIT. A weight
+rounded to one part alone would give sqrt(2)."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():
+    pytest.skip("no GPU", allow_module_level=True)
+
+from crack_detection_federatedlearning_grpc_amd import ops  # noqa: E402
+
+DEV = torch.device("cuda")
+BF, HF = torch.bfloat16, torch.float16
+LIMIT = 1.1
+
+
+def rnd(shape, dt, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(dt).to(DEV)
+
+
+def definition(q, k, v, go, ok=None):
+    """out, dq, dk, dv in 64 bits; ok: pairs that are allowed, (B, 1, Sq, Sk) or fewer axes."""
+    B, Sq, Hq, D = q.shape
+    Hkv = k.shape[2]
+    G = Hq // Hkv
+    Q, K, V, g = (t.double().transpose(1, 2).contiguous() for t in (q, k, v, go))
+    K, V = K.repeat_interleave(G, 1), V.repeat_interleave(G, 1)
+    s = Q @ K.transpose(2, 3) / math.sqrt(D)
+    if ok is not None:
+        s = s.masked_fill(~ok, -math.inf)
+    p = torch.softmax(s, 3)
+    o = p @ V
+    ds = p * (g @ V.transpose(2, 3) - (g * o).sum(3, keepdim=True)) / math.sqrt(D)
+    dk, dv = (t.unflatten(1, (Hkv, G)).sum(2) for t in (ds.transpose(2, 3) @ Q, p.transpose(2, 3) @ g))
+    return [t.transpose(1, 2) for t in (o, ds @ K, dk, dv)]
+
+
+def excess(q, k, v, go, ok=None, **kw):
+    """error over that of rounding the results, of out, dq, dk and dv"""
+    want = definition(q, k, v, go, ok)
+    ins = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = ops.attention(*ins, **kw)
+    got = [out.detach(), *torch.autograd.grad(out, ins, go)]
+    r = []
+    for g, w in zip(got, want):
+        assert torch.isfinite(w.to(q.dtype)).all()                   # the results themselves are in the type's range
+        r.append(float((g.double() - w).norm() / (w.to(q.dtype).double() - w).norm()))
+    return dict(zip(("out", "dq", "dk", "dv"), r))
+
+
+def check(q, k, v, go, ok=None, **kw):
+    e = excess(q, k, v, go, ok, **kw)
+    assert all(x <= LIMIT for x in e.values()), e
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("kind", ["plain", "causal", "lengths", "mask"])
+@pytest.mark.parametrize("D", [32, 64, 80, 128])
+def test_many_pairs_are_as_accurate_as_few(D, kind, dt):
+    """More than 2^24 pairs of a query and a key: the weights and dS are as exact as in a small call."""
+    B, S, Hq, Hkv = 4, 1100, 4, 2
+    assert B * Hq * S * S > 1 << 24
+    q, k, v, go = (rnd((B, S, h, D), dt, n) for n, h in enumerate((Hq, Hkv, Hkv, Hq)))
+    i = torch.arange(S, device=DEV)
+    if kind == "causal":
+        check(q, k, v, go, i <= i[:, None], causal=True)
+    elif kind == "lengths":
+        n = torch.tensor([S, 900, 333, 1], dtype=torch.int32, device=DEV)
+        check(q, k, v, go, (i < n[:, None])[:, None, None], lengths=n)
+    elif kind == "mask":
+        m = (torch.rand(S, S, generator=torch.Generator().manual_seed(9)) < 0.6).to(DEV)
+        check(q, k, v, go, m, mask=m)
+    else:
+        check(q, k, v, go)
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_an_image_alone_and_in_a_large_batch(dt):
+    """The number of images does not decide how exact a row is: an image's results in a batch are those of the image
+    alone but for the order of fp32 sums, so that few of them round to another value."""
+    B, S, H, D = 48, 640, 2, 64
+    q, k, v, go = (rnd((B, S, H, D), dt, n) for n in range(4))
+
+    def run(n):
+        ins = [t[:n].detach().requires_grad_() for t in (q, k, v)]
+        out = ops.attention(*ins)
+        return [t[:1] for t in (out.detach(), *torch.autograd.grad(out, ins, go[:n]))]
+
+    assert H * S * S < 1 << 24 < B * H * S * S
+    for name, a, b in zip(("out", "dq", "dk", "dv"), run(1), run(B)):
+        # a sum in another order differs by less than a 2^-9th of a half step here: a value in 2^8 rounds elsewhere
+        assert float((a != b).double().mean()) <= 2 ** -5, name
