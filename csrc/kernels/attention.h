@@ -26,6 +26,7 @@ typedef _Float16 h8v __attribute__((ext_vector_type(8)));
 typedef _Float16 h2v __attribute__((ext_vector_type(2)));
 
 struct BF16 {
+  static constexpr bool NARROW = false;         // fp32's exponents: nothing that is finite leaves the range
   static constexpr short INF = 0x7f80, ONE = 0x3f80;
   static CFL_DEVICE f16v mma(const s8v& a, const s8v& b, const f16v& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8v, a), __builtin_bit_cast(bf8v, b), c, 0, 0,
@@ -37,6 +38,7 @@ struct BF16 {
 };
 
 struct FP16 {
+  static constexpr bool NARROW = true;
   static constexpr short INF = 0x7c00, ONE = 0x3c00;
   static CFL_DEVICE f16v mma(const s8v& a, const s8v& b, const f16v& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
@@ -256,6 +258,49 @@ CFL_DEVICE float max_halves(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
   return fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
 }
+
+// dS as fp16 operands. ds = p (dp - delta) is about |do| sqrt(D) / Sk: below the normal range (2^-14) where the gradients,
+// sums of many, are in it, or above 65,504 where they are not. A lane holds ds of one row (dq) or one key (dk), and its
+// sums are that row's or key's: so they carry a power of two, f = 2^ef, as a softmax carries its maximum, and are divided
+// by it when they are stored. f starts so high that any ds which counts (2^-59 and more) brings it down; from then on the
+// largest ds so far is 2^-4 to 2, and what two parts cannot hold is below 2^-21 of it. Whether one has reached 2 is a bit
+// of the packed values: 4 operations for 16 of them, and a branch that is seldom taken (16 images x 8 heads x 1,024 tokens
+// of 64 channels: dq 82 -> 88 us, dk and dv 123 -> 134).
+template <class T>
+struct Fit {
+  float f, ef;
+  CFL_DEVICE void start() {
+    f = T::NARROW ? 0x1p60f : 1.f;
+    ef = T::NARROW ? 60.f : 0.f;
+  }
+  // x: 16 of the lane's ds times f -> ds; lower(g): called where f falls, to scale the lane's sums by g (1: not this
+  // lane's). What a lane does goes by its own values alone.
+  template <bool FINE, class F>
+  CFL_DEVICE void pack(f16v& x, Packed<T, FINE>* ds, const F& lower) {
+    ds[0].set(x, 0);
+    ds[1].set(x, 1);
+    if constexpr (T::NARROW) {
+      const u4v a = __builtin_bit_cast(u4v, ds[0].hi), b = __builtin_bit_cast(u4v, ds[1].hi);
+      const uint32_t any = (a[0] | a[1] | a[2]) | (a[3] | b[0] | b[1]) | (b[2] | b[3]);
+      if (__any((any & 0x40004000u) != 0)) {
+        float mx = fabsf(x[0]);                            // NaN is passed over; an infinity stays one and lowers nothing
+#pragma unroll
+        for (int e = 1; e < 16; ++e) mx = fmaxf(mx, fabsf(x[e]));
+        mx = max_halves(mx);
+        const int down = mx >= 2.f && mx < INFINITY ? -3 - __builtin_amdgcn_frexp_expf(mx) : 0;
+        const float g = ldexpf(1.f, down);
+        f *= g;
+        ef += (float)down;
+        lower(g);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] *= g;
+        ds[0].set(x, 0);
+        ds[1].set(x, 1);
+      }
+    }
+  }
+  CFL_DEVICE float undo(float mul) const { return T::NARROW ? mul / f : mul; }
+};
 
 // Which of `n` blocks of an (image, key head), which of bhn of those and which of `splits` parts this workgroup is.
 // Where all blocks have the same work, XCD by XCD: the blocks that read one head's tokens share an L2 (16 heads, 4,096

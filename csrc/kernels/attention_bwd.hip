@@ -134,10 +134,13 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
   };
 
   f16v acc[ND][QT];
+  Fit<T> fit[QT];
   const float sc = p.scale * LOG2E;
   const TransAt<DP> ta(lane);
   auto walk = [&](auto safe) {
     constexpr bool SAFE = decltype(safe)::value;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) fit[t].start();
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -207,7 +210,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
 #pragma unroll
           for (int u = 0; u < QT; ++u) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[u][e] = exp2_(fmaf(s[u][e], sc, -lse[u]));
+            for (int e = 0; e < 16; ++e) s[u][e] = exp2_(fmaf(s[u][e], sc, fit[u].ef - lse[u]));   // f p: it is only in dS
             if (MASK && part) {
               const uint32_t w = (uint32_t)(cur[u] >> (32 * k)) >> (4 * h);
 #pragma unroll
@@ -223,8 +226,12 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
               const float ds = s[u][e] * dp[u][e];
               s[u][e] = SAFE && s[u][e] == 0.f ? 0.f : ds;
             }
-            db[u][0].set(s[u], 0);
-            db[u][1].set(s[u], 1);
+            fit[u].pack(s[u], db[u], [&](float g) {
+#pragma unroll
+              for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[d][u][e] *= g;
+            });
           }
           if (DP == 128) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -268,12 +275,12 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
     if (p.splits > 1) {
       const int64_t part = ((int64_t)sp * bhn + bh) * p.M + rb * BR + (wid * QT + u) * 32 + c;
 #pragma unroll
-      for (int d = 0; d < ND; ++d) store_part<DP>(p.ws_o + part * DP, acc[d][u], p.scale, d, h, ok);
+      for (int d = 0; d < ND; ++d) store_part<DP>(p.ws_o + part * DP, acc[d][u], fit[u].undo(p.scale), d, h, ok);
       continue;
     }
     bf16_t* o = reinterpret_cast<bf16_t*>(p.dq.p) + b * p.dq.sb + ri[u] * p.dq.ss + (hk * p.G + rg[u]) * p.dq.sh;
 #pragma unroll
-    for (int d = 0; d < ND; ++d) store_row<T>(o, acc[d][u], p.scale, d, p.D, h, ok);
+    for (int d = 0; d < ND; ++d) store_row<T>(o, acc[d][u], fit[u].undo(p.scale), d, p.D, h, ok);
   }
 }
 
@@ -396,10 +403,13 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
   };
 
   f16v dk[ND][KQ], dv[ND][KQ];
+  Fit<T> fit[KQ];
   const float sc = p.scale * LOG2E;
   const TransAt<DP> ta(lane);
   auto walk = [&](auto safe) {
     constexpr bool SAFE = decltype(safe)::value;
+#pragma unroll
+    for (int u = 0; u < KQ; ++u) fit[u].start();
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -495,10 +505,15 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             dp[u][e] *= s[u][e];
+            if constexpr (T::NARROW) dp[u][e] *= fit[u].f;
             if constexpr (SAFE) dp[u][e] = s[u][e] == 0.f ? 0.f : dp[u][e];
           }
-          db[u][0].set(dp[u], 0);
-          db[u][1].set(dp[u], 1);
+          fit[u].pack(dp[u], db[u], [&](float g) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) dk[d][u][e] *= g;
+          });
         }
         if (VL) __builtin_amdgcn_sched_barrier(0);
         auto add_dv = [&]() {
@@ -566,14 +581,14 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
       const int64_t part = ((int64_t)sp * bhn + bh) * p.Sk + key, half = (int64_t)p.kv_splits * bhn * p.Sk;
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        store_part<DP>(p.ws_kv + part * DP, dk[d][u], p.scale, d, h, key < len);
+        store_part<DP>(p.ws_kv + part * DP, dk[d][u], fit[u].undo(p.scale), d, h, key < len);
         store_part<DP>(p.ws_kv + (half + part) * DP, dv[d][u], 1.f, d, h, key < len);
       }
       continue;
     }
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
-      if (p.dk.p) store_row<T>(ko, dk[d][u], p.scale, d, p.D, h, key < p.Sk, nullptr, key >= len);
+      if (p.dk.p) store_row<T>(ko, dk[d][u], fit[u].undo(p.scale), d, p.D, h, key < p.Sk, nullptr, key >= len);
       if (p.dv.p) store_row<T>(vo, dv[d][u], 1.f, d, p.D, h, key < p.Sk, nullptr, key >= len);
     }
   }

@@ -99,3 +99,57 @@ def test_an_image_alone_and_in_a_large_batch(dt):
     for name, a, b in zip(("out", "dq", "dk", "dv"), run(1), run(B)):
         # a sum in another order differs by less than a 2^-9th of a half step here: a value in 2^8 rounds elsewhere
         assert float((a != b).double().mean()) <= 2 ** -5, name
+
+
+# -------------------------------------------------------------------------------- float16: its range is 2^-24 .. 65,504
+DS = [(1, 1024, 4096, 2, 1, 64), (1, 256, 1024, 2, 2, 32), (1, 2048, 8192, 1, 1, 16), (2, 300, 300, 2, 2, 128),
+      (2, 20, 900, 2, 1, 96)]
+
+
+@pytest.mark.parametrize("kind", ["plain", "causal", "mask"])
+@pytest.mark.parametrize("power", [-12, -8, 0, 7])
+@pytest.mark.parametrize("shape", DS)
+def test_float16_gradients_of_any_magnitude(shape, power, kind):
+    """dS is about |go| sqrt(D) / Sk: far below float16's normal range where dq and dk, sums of many, are in it."""
+    B, Sq, Sk, Hq, Hkv, D = shape
+    q, k, v, go = (rnd((B, n, h, D), HF, i) for i, (n, h) in enumerate(((Sq, Hq), (Sk, Hkv), (Sk, Hkv), (Sq, Hq))))
+    go = go * 2.0 ** power
+    if kind == "causal":
+        ok = torch.arange(Sk, device=DEV) <= torch.arange(Sq, device=DEV)[:, None] + Sk - Sq
+        check(q, k, v, go, ok, causal=True)
+    elif kind == "mask":
+        m = (torch.rand(Sq, Sk, generator=torch.Generator().manual_seed(9)) < 0.6).to(DEV)
+        check(q, k, v, go, m, mask=m)
+    else:
+        check(q, k, v, go)
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_float16_ds_above_the_largest_number(D):
+    """p (dp - delta) passes 65,504, dq and dk do not."""
+    q, k, v, go = (rnd((1, n, 2, D), HF, i) for i, n in enumerate((16, 4, 4, 16)))
+    q, k, v, go = q * 0.1, k * 0.1, v * 16, go * 2048
+    w = go.double().transpose(1, 2) @ v.double().transpose(1, 2).transpose(2, 3)
+    assert float((w - w.mean(3, keepdim=True)).abs().max()) / 4 > 65504          # p is about 1 / 4
+    check(q, k, v, go)
+
+
+@pytest.mark.parametrize("kind", ["plain", "causal"])
+@pytest.mark.parametrize("up", [True, False])
+@pytest.mark.parametrize("D", [32, 64, 80, 128])
+def test_float16_magnitudes_that_change_along_a_walk(D, up, kind):
+    """Values and gradients that grow, or fall, by 2^16 from the first token to the last: every query's dq and every
+    key's dk and dv is as exact as its own size allows."""
+    S = 700
+    q, k, v, go = (rnd((1, S, 2, D), HF, i) for i in range(4))
+    s = 2.0 ** (torch.linspace(-10, 6, S, device=DEV) * (1 if up else -1) - (0 if up else 4))[:, None, None]
+    v, go = (v * s).to(HF), (go * s).to(HF)
+    ok = torch.arange(S, device=DEV) <= torch.arange(S, device=DEV)[:, None] if kind == "causal" else None
+    want = definition(q, k, v, go, ok)
+    ins = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = ops.attention(*ins, causal=kind == "causal")
+    for name, g, w in zip(("dq", "dk", "dv"), torch.autograd.grad(out, ins, go), want[1:]):
+        size = w.abs().amax(3, keepdim=True)                                      # a token's own magnitude
+        size = torch.where(size == 0, torch.ones_like(size), size)
+        off, least = (g.double() - w) / size, (w.to(HF).double() - w) / size
+        assert float(off.norm() / least.norm()) <= LIMIT, (name, float(off.norm() / least.norm()))
