@@ -257,11 +257,12 @@ void backward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, con
   ok(attn_bwd(p, stream()), "attention backward");
 }
 
-at::Tensor natural_lse(const at::Tensor& lse2, const Shape& s) {
+at::Tensor natural_lse(const at::Tensor& lse2, const Shape& s, bool fp16) {
   const int64_t G = s.Hq / s.Hkv;
   const at::Tensor t = lse2.view({s.B, s.Hkv, s.Sq, G}).permute({0, 1, 3, 2}).reshape({s.B, s.Hq, s.Sq});
   const double inf = std::numeric_limits<double>::infinity();
-  return at::where(t == inf, at::scalar_tensor(-inf, t.options()), t * 0.6931471805599453);
+  return at::where(t == inf, at::scalar_tensor(-inf, t.options()),
+                   (fp16 ? t + ATTN_FP16_P_UP : t) * 0.6931471805599453);
 }
 
 void put_meta(AutogradContext* ctx, const Shape& s, bool causal, double scale, const PackedMask& pm) {
@@ -362,7 +363,7 @@ struct AttentionQkvFn : torch::autograd::Function<AttentionQkvFn> {
 
 py::object result(const at::Tensor& out, const at::Tensor& lse2, const Shape& s, bool return_lse) {
   if (!return_lse) return py::cast(out);
-  return py::make_tuple(out, natural_lse(lse2, s));
+  return py::make_tuple(out, natural_lse(lse2, s, out.scalar_type() == at::kHalf));
 }
 
 py::object attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const OptT& mask,

@@ -27,6 +27,7 @@ typedef _Float16 h2v __attribute__((ext_vector_type(2)));
 
 struct BF16 {
   static constexpr bool NARROW = false;         // fp32's exponents: nothing that is finite leaves the range
+  static constexpr float UP = 0.f, P_UP = 0.f;
   static constexpr short INF = 0x7f80, ONE = 0x3f80;
   static CFL_DEVICE f16v mma(const s8v& a, const s8v& b, const f16v& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8v, a), __builtin_bit_cast(bf8v, b), c, 0, 0,
@@ -38,7 +39,12 @@ struct BF16 {
 };
 
 struct FP16 {
+  // Its numbers end at 65,504 and lose bits below 2^-14, so the softmax weights are held times a power of two, in the
+  // exponent, where it costs nothing. Forward 2^UP: weights down to 2^-21 of the row's largest keep their bits, and
+  // those that lag the maximum (attention.hip SLACK) reach 2^15. Backward, where they are normalised, 2^P_UP: down to
+  // 2^-28, and the largest is 2^14. lse2 is kept less P_UP, so that exp2(s - lse2) is P times it.
   static constexpr bool NARROW = true;
+  static constexpr float UP = 7.f, P_UP = ATTN_FP16_P_UP;
   static constexpr short INF = 0x7c00, ONE = 0x3c00;
   static CFL_DEVICE f16v mma(const s8v& a, const s8v& b, const f16v& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
@@ -57,6 +63,10 @@ enum Kind { ATTN_PLAIN = 0, ATTN_CAUSAL = 1, ATTN_MASK = 2 };
 CFL_DEVICE int rowof(int e, int h) { return (e & 3) + 8 * (e >> 2) + 4 * h; }
 
 CFL_DEVICE float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// 2^-P_UP
+template <class T>
+CFL_DEVICE constexpr float p_undo() { return T::NARROW ? 1.f / (1 << (int)T::P_UP) : 1.f; }
 
 // value of the lane 32 away
 CFL_DEVICE float other_half(float v) {
@@ -270,8 +280,8 @@ template <class T>
 struct Fit {
   float f, ef;
   CFL_DEVICE void start() {
-    f = T::NARROW ? 0x1p60f : 1.f;
-    ef = T::NARROW ? 60.f : 0.f;
+    f = T::NARROW ? 0x1p46f : 1.f;                         // P has P_UP = 14 more
+    ef = T::NARROW ? 46.f : 0.f;
   }
   // x: 16 of the lane's ds times f -> ds; lower(g): called where f falls, to scale the lane's sums by g (1: not this
   // lane's). What a lane does goes by its own values alone.
@@ -299,7 +309,7 @@ struct Fit {
       }
     }
   }
-  CFL_DEVICE float undo(float mul) const { return T::NARROW ? mul / f : mul; }
+  CFL_DEVICE float undo(float mul) const { return T::NARROW ? mul / f * p_undo<T>() : mul; }
 };
 
 // Which of `n` blocks of an (image, key head), which of bhn of those and which of `splits` parts this workgroup is.

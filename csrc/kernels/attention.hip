@@ -25,8 +25,8 @@ namespace {
 
 using namespace attn;
 
-// row maxima may lag the running maximum by 2^SLACK: P then reaches 2^SLACK (exact in both types' range, the relative
-// precision is the same) and most tiles rescale nothing
+// row maxima may lag the running maximum by 2^SLACK: P then reaches 2^SLACK (times 2^UP: in both types' range, the
+// relative precision is the same) and most tiles rescale nothing
 constexpr float SLACK = 8.f;
 
 // up to this many rows the four waves of a block split the keys of a tile, beyond it the rows
@@ -234,7 +234,7 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
 #pragma unroll
               for (int e = 0; e < 16; ++e) acc[d][u][e] *= al;
           }
-          const float ms = m[u] == -INFINITY ? 0.f : m[u];
+          const float ms = (m[u] == -INFINITY ? 0.f : m[u]) - T::UP;
           float sum = 0.f;
 #pragma unroll
           for (int k = 0; k < NK; ++k) {
@@ -358,7 +358,7 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
       store_row<T>(o, acc[d][u], inv, d, p.D, h, ok, rest);
     }
     if (ok && h == 0 && p.lse2)
-      p.lse2[row] = l[u] == 0.f ? INFINITY : m[u] + __builtin_amdgcn_logf(l[u]);
+      p.lse2[row] = l[u] == 0.f ? INFINITY : m[u] + __builtin_amdgcn_logf(l[u]) - (T::UP + T::P_UP);
   }
 }
 
@@ -410,7 +410,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnParams p) {
       *reinterpret_cast<uint2*>(p.o_rest + at) = make_uint2(T::pack2(a0 - T::lo(w.x), a1 - T::hi(w.x)),
                                                             T::pack2(a2 - T::lo(w.y), a3 - T::hi(w.y)));
   }
-  if (d == 0 && p.lse2) p.lse2[row] = l == 0.f ? INFINITY : mn + __builtin_amdgcn_logf(l);
+  if (d == 0 && p.lse2) p.lse2[row] = l == 0.f ? INFINITY : mn + __builtin_amdgcn_logf(l) - (T::UP + T::P_UP);
 }
 
 // mask bytes -> words: one wave per (32 mask rows, 64 keys), all of its loads under way together

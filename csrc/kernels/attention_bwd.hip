@@ -11,8 +11,8 @@
 // leave one wave a SIMD: slower at every width but 32 (128 channels 1,045 us against 953 then).
 // delta is taken from the output before its rounding (o + what that took away): with few keys dp - delta cancels, and a
 // rounded o would leave its whole step there.
-// Rounding: P and dS enter the second products in two parts of the inputs' type (attn_fine); everything else is fp32
-// until the gradients are rounded once.
+// Rounding: P and dS enter the second products in two parts of the inputs' type (attn_fine), in fp16 times powers of two
+// that keep them in its range (attention.h FP16, Fit); everything else is fp32 until the gradients are rounded once.
 #include <algorithm>
 
 #include "attention.h"
@@ -368,7 +368,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
       dma16(rq, in ? oq : CFL_OOB, dst + NT * 8 * n);
       dma16(rg, in ? og : CFL_OOB, dst + TILE + NT * 8 * n);
     }
-    // rows past the last read 0 everywhere: p = 1, do = 0, ds = 0
+    // rows past the last read 0 everywhere: p is finite, do = 0, ds = 0
     if (wid < 2) {
       const u4v rs = rsrc((wid ? p.delta : p.lse2) + (int64_t)bh * p.M + r0);
       dma4(rs, lane < imin(rem, RT) ? 4u * lane : CFL_OOB, &sstat[buf][wid][0]);
@@ -582,14 +582,14 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
         store_part<DP>(p.ws_kv + part * DP, dk[d][u], fit[u].undo(p.scale), d, h, key < len);
-        store_part<DP>(p.ws_kv + (half + part) * DP, dv[d][u], 1.f, d, h, key < len);
+        store_part<DP>(p.ws_kv + (half + part) * DP, dv[d][u], p_undo<T>(), d, h, key < len);
       }
       continue;
     }
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
       if (p.dk.p) store_row<T>(ko, dk[d][u], fit[u].undo(p.scale), d, p.D, h, key < p.Sk, nullptr, key >= len);
-      if (p.dv.p) store_row<T>(vo, dv[d][u], 1.f, d, p.D, h, key < p.Sk, nullptr, key >= len);
+      if (p.dv.p) store_row<T>(vo, dv[d][u], p_undo<T>(), d, p.D, h, key < p.Sk, nullptr, key >= len);
     }
   }
 }

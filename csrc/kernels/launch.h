@@ -640,7 +640,8 @@ struct AttnParams {
   AttnTensor q, k, v, o;            // o: forward output
   bf16_t* o_rest;                   // o before its rounding less o, laid out like o; kept for the backward (or nullptr)
   AttnTensor go, dq, dk, dv;        // backward
-  float* lse2;                      // [B][Hkv][M] log2 of the row's exp2 sum (+inf: empty row); saved for the backward
+  float* lse2;                      // [B][Hkv][M] log2 of the row's exp2 sum (+inf: empty row), of fp16 calls less
+                                    // ATTN_FP16_P_UP; saved for the backward
   float* delta;                     // [B][Hkv][M] -sum(do o), workspace of the backward
   AttnMask mask;
   const int* lengths;               // [B] valid keys or nullptr
@@ -666,6 +667,7 @@ struct AttnMaskArgs {
 };
 
 int attn_mask_bits(const AttnMaskArgs& a, hipStream_t st);
+constexpr int ATTN_FP16_P_UP = 14;                   // attention.h FP16
 constexpr int64_t ATTN_MAX_BLOCKS = 0xffffff;        // of 256 threads: a launch has fewer than 2^32
 bool attn_fine();                                    // P and dS in two 16-bit parts
 int attn_splits(int B, int Hkv, int M, int Sk);      // key splits of a forward call (1: no workspace)

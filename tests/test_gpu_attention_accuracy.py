@@ -102,6 +102,26 @@ def test_an_image_alone_and_in_a_large_batch(dt):
 
 
 # -------------------------------------------------------------------------------- float16: its range is 2^-24 .. 65,504
+@pytest.mark.parametrize("Sq,Sk,D", [(64, 65536, 32), (16, 262144, 16), (200, 40000, 128)])
+def test_float16_weights_of_long_keys(Sq, Sk, D):
+    """Weights of 1 / Sk are below float16's normal range, dv is not."""
+    q, k, v, go = (rnd((1, n, 1, D), HF, i) for i, n in enumerate((Sq, Sk, Sk, Sq)))
+    e = excess(q, k, v, go * 64)
+    assert e["out"] <= LIMIT and e["dv"] <= LIMIT, e
+
+
+@pytest.mark.parametrize("Sq", [1, 70])
+def test_float16_weights_far_below_the_largest(Sq):
+    """One key that outweighs all others by 2^20 and has no value: the output is what the others say."""
+    D = 32
+    q, k, v, go = (rnd((1, n, 1, D), HF, i) for i, n in enumerate((Sq, 65, 65, Sq)))
+    q[..., 0], k[..., 0] = 8, 0
+    k[:, 0], v[:, 0] = 0, 0
+    k[:, 0, :, 0] = 20 * math.log(2) * math.sqrt(D) / 8
+    e = excess(q, k, v * 1000, go)
+    assert e["out"] <= LIMIT and e["dv"] <= LIMIT, e
+
+
 DS = [(1, 1024, 4096, 2, 1, 64), (1, 256, 1024, 2, 2, 32), (1, 2048, 8192, 1, 1, 16), (2, 300, 300, 2, 2, 128),
       (2, 20, 900, 2, 1, 96)]
 
