@@ -27,7 +27,7 @@ typedef _Float16 h2v __attribute__((ext_vector_type(2)));
 
 struct BF16 {
   static constexpr bool NARROW = false;         // fp32's exponents: nothing that is finite leaves the range
-  static constexpr float UP = 0.f, P_UP = 0.f;
+  static constexpr float UP = 0.f, P_UP = 0.f, REST = 1.f;
   static constexpr short INF = 0x7f80, ONE = 0x3f80;
   static CFL_DEVICE f16v mma(const s8v& a, const s8v& b, const f16v& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8v, a), __builtin_bit_cast(bf8v, b), c, 0, 0,
@@ -42,9 +42,10 @@ struct FP16 {
   // Its numbers end at 65,504 and lose bits below 2^-14, so the softmax weights are held times a power of two, in the
   // exponent, where it costs nothing. Forward 2^UP: weights down to 2^-21 of the row's largest keep their bits, and
   // those that lag the maximum (attention.hip SLACK) reach 2^15. Backward, where they are normalised, 2^P_UP: down to
-  // 2^-28, and the largest is 2^14. lse2 is kept less P_UP, so that exp2(s - lse2) is P times it.
+  // 2^-28, and the largest is 2^14. lse2 is kept less P_UP, so that exp2(s - lse2) is P times it. What the rounding of
+  // the output took away, at most 2^-11 of it, is kept times REST.
   static constexpr bool NARROW = true;
-  static constexpr float UP = 7.f, P_UP = ATTN_FP16_P_UP;
+  static constexpr float UP = 7.f, P_UP = ATTN_FP16_P_UP, REST = 2048.f;
   static constexpr short INF = 0x7c00, ONE = 0x3c00;
   static CFL_DEVICE f16v mma(const s8v& a, const s8v& b, const f16v& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
@@ -195,7 +196,7 @@ struct Packed {
 
 // 32 channels 32 * dt .. + 31 of one token row per lane pair (c, c + 32): four quads each, exchanged between the
 // halves so that a lane stores 16 contiguous bytes (lane half h: channels 16s + 8h .. + 7). rest: if given, what the
-// rounding took away, rounded itself. zero: zeros are stored, whatever v holds.
+// rounding took away, times REST, rounded itself. zero: zeros are stored, whatever v holds.
 template <class T>
 CFL_DEVICE void store_row(bf16_t* row, const f16v& v, float mul, int dt, int D, int h, bool ok,
                           bf16_t* rest = nullptr, bool zero = false) {
@@ -206,7 +207,7 @@ CFL_DEVICE void store_row(bf16_t* row, const f16v& v, float mul, int dt, int D, 
     for (int j = 0; j < 4; ++j) {
       const float a = zero ? 0.f : v[8 * s + 2 * j] * mul, b = zero ? 0.f : v[8 * s + 2 * j + 1] * mul;
       w[j] = T::pack2(a, b);
-      x[j] = T::pack2(a - T::lo(w[j]), b - T::hi(w[j]));
+      x[j] = T::pack2((a - T::lo(w[j])) * T::REST, (b - T::hi(w[j])) * T::REST);
     }
     const int d = 32 * dt + 16 * s + 8 * h;
     const auto p = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);

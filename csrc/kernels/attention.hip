@@ -407,8 +407,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnParams p) {
     const uint2 w = make_uint2(T::pack2(a0, a1), T::pack2(a2, a3));
     *reinterpret_cast<uint2*>(reinterpret_cast<bf16_t*>(p.o.p) + at) = w;
     if (p.o_rest)
-      *reinterpret_cast<uint2*>(p.o_rest + at) = make_uint2(T::pack2(a0 - T::lo(w.x), a1 - T::hi(w.x)),
-                                                            T::pack2(a2 - T::lo(w.y), a3 - T::hi(w.y)));
+      *reinterpret_cast<uint2*>(p.o_rest + at) =
+          make_uint2(T::pack2((a0 - T::lo(w.x)) * T::REST, (a1 - T::hi(w.x)) * T::REST),
+                     T::pack2((a2 - T::lo(w.y)) * T::REST, (a3 - T::hi(w.y)) * T::REST));
   }
   if (d == 0 && p.lse2) p.lse2[row] = l == 0.f ? INFINITY : mn + __builtin_amdgcn_logf(l) - (T::UP + T::P_UP);
 }

@@ -71,7 +71,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
       }
 #pragma unroll
       for (int x = 0; x < 4; ++x)
-        dl = fmaf(T::lo(wg[x]), T::lo(wo[x]) + T::lo(wr[x]), fmaf(T::hi(wg[x]), T::hi(wo[x]) + T::hi(wr[x]), dl));
+        dl = fmaf(T::lo(wg[x]), fmaf(T::lo(wr[x]), 1.f / T::REST, T::lo(wo[x])),
+                  fmaf(T::hi(wg[x]), fmaf(T::hi(wr[x]), 1.f / T::REST, T::hi(wo[x])), dl));
       qf[t][kk] = __builtin_bit_cast(s8v, wq);
       gf[t][kk] = __builtin_bit_cast(s8v, wg);
     }

@@ -638,7 +638,8 @@ struct AttnMask {
 
 struct AttnParams {
   AttnTensor q, k, v, o;            // o: forward output
-  bf16_t* o_rest;                   // o before its rounding less o, laid out like o; kept for the backward (or nullptr)
+  bf16_t* o_rest;                   // o before its rounding less o, of fp16 calls times 2^11, laid out like o; kept for
+                                    // the backward (or nullptr)
   AttnTensor go, dq, dk, dv;        // backward
   float* lse2;                      // [B][Hkv][M] log2 of the row's exp2 sum (+inf: empty row), of fp16 calls less
                                     // ATTN_FP16_P_UP; saved for the backward

@@ -122,6 +122,14 @@ def test_float16_weights_far_below_the_largest(Sq):
     assert e["out"] <= LIMIT and e["dv"] <= LIMIT, e
 
 
+@pytest.mark.parametrize("power", [-11, -13, -15])
+@pytest.mark.parametrize("Sk", [4, 64, 700])
+def test_float16_small_outputs(Sk, power):
+    """dp - delta cancels to what the output's rounding took away, and that is below the type's smallest number."""
+    q, k, v, go = (rnd((1, n, 2, 64), HF, i) for i, n in enumerate((200, Sk, Sk, 200)))
+    check(q, k * 0.3, v * 2.0 ** power, go * 64)
+
+
 DS = [(1, 1024, 4096, 2, 1, 64), (1, 256, 1024, 2, 2, 32), (1, 2048, 8192, 1, 1, 16), (2, 300, 300, 2, 2, 128),
       (2, 20, 900, 2, 1, 96)]
 
