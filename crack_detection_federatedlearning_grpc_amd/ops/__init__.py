@@ -19,6 +19,9 @@ Layers of a transformer block over the same maps, their pixels read as tokens (B
     q = rotary(q, positions, dims)        # rotary positions, 1-4 axes         (rotary.py;    kernel: rotary.hip)
     y = attention(q, k, v, ...)           # softmax(q k^T) v, masked / causal  (attention.py; kernel: attention*.hip)
     y = self_attention2d(x, ...)          # the block of them with 1x1 convs   (block.py)
+
+These take tensors in memory only: a call that is being traced (torch.jit.trace, make_fx) or gets fake, functional or zero
+tensors raises NotImplementedError.
 """
 from __future__ import annotations
 

@@ -6,7 +6,9 @@
 #include "block_ops.h"
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cmath>
 #include <limits>
@@ -39,9 +41,26 @@ bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
   return false;
 }
 
+// The kernels write through pointers. What records calls (jit.trace, make_fx) would see an allocation only and return
+// memory as it was found, what stands for a tensor without holding it (fake, functional, zero tensors) has no address.
+void check_eager(const char* what, std::initializer_list<const at::Tensor*> ts) {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  bool eager = !torch::jit::tracer::isTracing();
+  if (Modes::any_modes_set())
+    for (const Key k : {Key::FAKE, Key::PROXY, Key::FUNCTIONAL}) eager = eager && !Modes::get_mode(k).has_value();
+  for (const at::Tensor* t : ts)
+    if (t->defined())
+      eager = eager && t->has_storage() && !t->key_set().has(c10::DispatchKey::Functionalize) &&
+              t->storage().device() == t->device() && (t->numel() == 0 || t->const_data_ptr() != nullptr);
+  TORCH_CHECK_NOT_IMPLEMENTED(eager, what, ": runs on tensors in memory only; it cannot be traced, nor take fake, "
+                              "functional or zero tensors");
+}
+
 // A backward pass that is itself recorded (create_graph=True) would be taken for a constant by the next derivative.
-void once(const char* what) {
+void check_backward(const char* what, const at::Tensor& g) {
   TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), what, ": the backward pass cannot be differentiated");
+  check_eager(what, {&g});
 }
 
 void check_device(const at::Tensor& t, const at::Tensor& like, const char* name) {
@@ -108,6 +127,8 @@ Shape check_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor
     TORCH_CHECK_VALUE(lengths->dim() == 1 && lengths->size(0) == s.B, "attention: lengths must be (", s.B, ",), got ",
                       lengths->sizes());
   }
+  const at::Tensor none;
+  check_eager("attention", {&q, &k, &v, mask ? &*mask : &none, lengths ? &*lengths : &none});
   TORCH_CHECK(q.is_cuda(), "attention: q must be a device tensor");
   check_device(k, q, "attention: k");
   check_device(v, q, "attention: v");
@@ -295,7 +316,7 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
     return {out, sv.lse2};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    once("attention");
+    check_backward("attention", g[0]);
     const auto t = ctx->get_saved_variables();
     Shape s;
     bool causal;
@@ -335,7 +356,7 @@ struct AttentionQkvFn : torch::autograd::Function<AttentionQkvFn> {
     return {out, sv.lse2};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    once("attention_qkv");
+    check_backward("attention_qkv", g[0]);
     const auto t = ctx->get_saved_variables();
     Shape s;
     bool causal;
@@ -388,6 +409,7 @@ py::object attention_qkv(const at::Tensor& qkv, int64_t heads, std::optional<int
   TORCH_CHECK_VALUE(heads >= 1 && kv >= 1 && qkv.size(2) == heads + 2 * kv, "attention_qkv: qkv ", qkv.sizes(),
                     " does not hold ", heads, " query and 2 x ", kv, " key and value heads");
   const double sc = scale ? *scale : qkv.size(3) > 0 ? 1.0 / std::sqrt((double)qkv.size(3)) : 1.0;
+  check_eager("attention_qkv", {&qkv});
   const at::Tensor q = qkv.narrow(2, 0, heads), k = qkv.narrow(2, heads, kv), v = qkv.narrow(2, heads + kv, kv);
   const Shape s = check_attention(q, k, v, mask, lengths, sc);
   const c10::DeviceGuard guard(qkv.device());
@@ -463,7 +485,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     return ln_forward(x, wc, bc, eps);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    once("layer_norm");
+    check_backward("layer_norm", g[0]);
     const auto t = ctx->get_saved_variables();
     const at::Tensor &x = t[0], &w = t[1];
     const int64_t C = x.size(-1);
@@ -516,10 +538,11 @@ at::Tensor layer_norm(const at::Tensor& x, const OptT& weight, const OptT& bias,
       TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == C, "layer_norm: ", name, " must be (", C, ",), got ",
                         t->sizes());
     }
+  const at::Tensor w = weight ? *weight : at::Tensor(), b = bias ? *bias : at::Tensor();
+  check_eager("layer_norm", {&x, &w, &b});
   TORCH_CHECK(x.is_cuda(), "layer_norm: x must be a device tensor");
   if (weight) check_device(*weight, x, "layer_norm: weight");
   if (bias) check_device(*bias, x, "layer_norm: bias");
-  const at::Tensor w = weight ? *weight : at::Tensor(), b = bias ? *bias : at::Tensor();
   const c10::DeviceGuard guard(x.device());
   if (wants_grad({&x, &w, &b})) return LayerNormFn::apply(x, weight, bias, eps);
   return ln_forward(x, w.defined() ? w.contiguous() : w, b.defined() ? b.contiguous() : b, eps);
@@ -571,7 +594,7 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
     return rotary_run(x, pos, pl, false);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    once("rotary");
+    check_backward("rotary", g[0]);
     const auto t = ctx->get_saved_variables();
     const auto m = ctx->saved_data["plan"].toIntVector();
     const RotaryPlan pl{m[0], {m[1], m[2], m[3], m[4]}, ctx->saved_data["theta"].toDouble(), m[5] != 0, m[6] != 0};
@@ -605,6 +628,7 @@ at::Tensor rotary(const at::Tensor& x, const at::Tensor& pos, const std::vector<
   TORCH_CHECK_VALUE(!pos.requires_grad(), "rotary: positions have no gradient");
   constexpr int64_t top = (int64_t)1 << 31;
   TORCH_CHECK_VALUE(B < top && S < top && x.size(2) < top && x.size(3) < top, "rotary: too large: x ", x.sizes());
+  check_eager("rotary", {&x, &pos});
   TORCH_CHECK(x.is_cuda(), "rotary: x must be a device tensor");
   check_device(pos, x, "rotary: positions");
   pl.theta = theta;

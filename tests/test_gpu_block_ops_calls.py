@@ -1,0 +1,56 @@
+"""Calls of attention, rotary positions and layer norm that are unusual, not wrong, or that have to be refused (marked
+gpu)."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():
+    pytest.skip("no GPU", allow_module_level=True)
+
+from torch.fx.experimental.proxy_tensor import make_fx  # noqa: E402
+
+from crack_detection_federatedlearning_grpc_amd import ops  # noqa: E402
+
+DEV = torch.device("cuda")
+BF, FF = torch.bfloat16, torch.float32
+
+
+def rnd(shape, dt, seed):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dt).to(DEV)
+
+
+POS = torch.arange(6, dtype=torch.int32)[None].to(DEV)
+CALLS = {
+    "attention": (lambda t: ops.attention(t, t, t), (2, 6, 2, 32)),
+    "attention_qkv": (lambda t: ops.attention_qkv(t, 2), (2, 6, 6, 32)),
+    "layer_norm": (lambda t: ops.layer_norm(t), (6, 32)),
+    "rotary": (lambda t: ops.rotary(t, POS, (32,)), (2, 6, 2, 32)),
+}
+
+
+@pytest.fixture(params=list(CALLS))
+def call(request):
+    f, shape = CALLS[request.param]
+    return f, rnd(shape, BF, 0)
+
+
+def test_a_traced_backward_pass_is_refused(call):
+    """The graph was made by an ordinary call; its backward pass writes through pointers like the call itself."""
+    f, x = call
+    x.requires_grad_()
+    y = f(x)
+    go = torch.ones_like(y)
+    with pytest.raises(NotImplementedError, match="cannot be traced"):
+        make_fx(lambda g: torch.autograd.grad(y, x, g, retain_graph=True))(go)
+    with pytest.raises(NotImplementedError, match="zero tensors"):
+        torch.autograd.grad(y, x, torch._efficientzerotensor(y.shape, dtype=BF, device=DEV), retain_graph=True)
+    (a,), (b,) = (torch.autograd.grad(y, x, go, retain_graph=True) for _ in range(2))
+    assert torch.equal(a, b)
+
+
+def test_a_compiled_function_calls_them_eagerly(call):
+    """A compiler that meets the call breaks its graph there: the same result."""
+    f, x = call
+    g = torch.compile(lambda t: f(t * 2) + 1, backend="eager")
+    assert torch.equal(g(x), f(x * 2) + 1)
