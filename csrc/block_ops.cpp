@@ -625,7 +625,7 @@ at::Tensor rotary(const at::Tensor& x, const at::Tensor& pos, const std::vector<
                         (pos.dim() == 3 && pos.size(0) == A && (pos.size(1) == B || pos.size(1) == 1) &&
                          pos.size(2) == S),
                     "rotary: positions must be (", A, ", ", S, ") or (", A, ", ", B, ", ", S, "), got ", pos.sizes());
-  TORCH_CHECK_VALUE(!pos.requires_grad(), "rotary: positions have no gradient");
+  TORCH_CHECK_VALUE(!pos.requires_grad() && !pos._fw_grad(0).defined(), "rotary: positions have no gradient");
   constexpr int64_t top = (int64_t)1 << 31;
   TORCH_CHECK_VALUE(B < top && S < top && x.size(2) < top && x.size(3) < top, "rotary: too large: x ", x.sizes());
   check_eager("rotary", {&x, &pos});

@@ -90,3 +90,14 @@ def test_modes_that_only_watch_are_no_tracing(call):
     f, x = call
     with Watch(), pytest.raises(RuntimeError, match="device tensor"):
         f(x)
+
+
+def test_tangents_of_positions_are_refused():
+    """A forward-mode derivative along the positions would be lost."""
+    import torch.autograd.forward_ad as fwd
+    x, pos = torch.zeros(2, 5, 4, 32, dtype=BF), torch.zeros(2, 5)
+    with fwd.dual_level():
+        dual = fwd.make_dual(pos, torch.ones_like(pos))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="positions have no gradient"):
+                ops.rotary(x, dual, (16, 16))
