@@ -63,6 +63,9 @@ void check_backward(const char* what, const at::Tensor& g) {
   check_eager(what, {&g});
 }
 
+// the values of a tensor with a pending sign (the imaginary part of a conjugate), which memory does not show
+at::Tensor with_sign(const at::Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+
 void check_device(const at::Tensor& t, const at::Tensor& like, const char* name) {
   TORCH_CHECK(t.is_cuda(), name, " must be a device tensor");
   TORCH_CHECK(t.device() == like.device(), name, " must be on ", like.device(), ", is on ", t.device());
@@ -505,7 +508,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
       return r;
     }
     int64_t xs, gs;
-    const at::Tensor xr = rows_of(x, C, xs), gr = rows_of(g[0], C, gs);
+    const at::Tensor xr = rows_of(x, C, xs), gr = rows_of(with_sign(g[0]), C, gs);
     LayerNormParams p = ln_params(xr, w, C, ctx->saved_data["eps"].toDouble());
     p.x_stride = xs;
     p.gy = gr.data_ptr();
@@ -524,7 +527,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
   }
 };
 
-at::Tensor layer_norm(const at::Tensor& x, const OptT& weight, const OptT& bias, double eps) {
+at::Tensor layer_norm(const at::Tensor& x, OptT weight, OptT bias, double eps) {
   TORCH_CHECK_VALUE(x.dim() >= 1, "layer_norm: x must have at least one axis");
   type_code(x, "layer_norm: x");
   const int64_t C = x.size(-1);
@@ -544,8 +547,10 @@ at::Tensor layer_norm(const at::Tensor& x, const OptT& weight, const OptT& bias,
   if (weight) check_device(*weight, x, "layer_norm: weight");
   if (bias) check_device(*bias, x, "layer_norm: bias");
   const c10::DeviceGuard guard(x.device());
-  if (wants_grad({&x, &w, &b})) return LayerNormFn::apply(x, weight, bias, eps);
-  return ln_forward(x, w.defined() ? w.contiguous() : w, b.defined() ? b.contiguous() : b, eps);
+  if (weight) weight = with_sign(*weight);
+  if (bias) bias = with_sign(*bias);
+  if (wants_grad({&x, &w, &b})) return LayerNormFn::apply(with_sign(x), weight, bias, eps);
+  return ln_forward(with_sign(x), weight ? weight->contiguous() : w, bias ? bias->contiguous() : b, eps);
 }
 
 // ------------------------------------------------------------------------------------------------------- rotary
@@ -635,8 +640,8 @@ at::Tensor rotary(const at::Tensor& x, const at::Tensor& pos, const std::vector<
   pl.joint = joint;
   pl.interleaved = interleaved;
   const c10::DeviceGuard guard(x.device());
-  if (wants_grad({&x})) return RotaryFn::apply(x, pos, pl);
-  return rotary_run(x, pos, pl, false);
+  if (wants_grad({&x})) return RotaryFn::apply(x, with_sign(pos), pl);
+  return rotary_run(x, with_sign(pos), pl, false);
 }
 
 }  // namespace

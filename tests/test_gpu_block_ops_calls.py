@@ -54,3 +54,21 @@ def test_a_compiled_function_calls_them_eagerly(call):
     f, x = call
     g = torch.compile(lambda t: f(t * 2) + 1, backend="eager")
     assert torch.equal(g(x), f(x * 2) + 1)
+
+
+def test_pending_signs_are_read():
+    """The imaginary part of a conjugate is a view of the same memory with its sign pending."""
+    z = torch.randn(2, 6, dtype=torch.complex64, generator=torch.Generator().manual_seed(3)).to(DEV)
+    pos = z.conj().imag
+    assert pos.is_neg()
+    x = rnd((1, 6, 2, 32), FF, 1)
+    assert torch.equal(ops.rotary(x, pos, (16, 16)), ops.rotary(x, pos.clone(), (16, 16)))
+    one = z.view(12, 1).conj().imag                          # rows of one column, read at their stride
+    w, b = (t.detach().requires_grad_() for t in (one[0], one[1]))
+    assert w.is_neg() and one.is_neg()
+    y = ops.layer_norm(one, w, b)
+    u, v = (t.detach().clone().requires_grad_() for t in (w, b))
+    want = ops.layer_norm(one.clone(), u, v)
+    assert torch.equal(y, want)
+    for s, t in zip(torch.autograd.grad(y, (w, b), one), torch.autograd.grad(want, (u, v), one.clone())):
+        assert torch.equal(s, t)
