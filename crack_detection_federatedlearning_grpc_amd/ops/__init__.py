@@ -63,13 +63,21 @@ def _conv_fwd(xb: torch.Tensor, wp: torch.Tensor, bias: Optional[torch.Tensor], 
 class _Conv(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, transpose: bool):
+        if x.dim() != 4 or w.dim() != 4:
+            raise ValueError(f"x must be (B, H, W, C), w (kh, kw, ., .), got {tuple(x.shape)}, {tuple(w.shape)}")
         B, H, W, Cin = x.shape
         ks = w.shape[0]
-        N = w.shape[2] if transpose else w.shape[3]
+        N, w_in = w.shape[2:] if transpose else w.shape[2:][::-1]
         if ks not in (1, 3) or w.shape[1] != ks or (transpose and ks != 3):
             raise ValueError("supported: 3x3 (Conv2D / Conv2DTranspose) and 1x1 Conv2D, stride 1")
+        if w_in != Cin:                                    # the kernels read Cin x N weights whatever w holds
+            raise ValueError(f"w takes {w_in} channels, x has {Cin}")
         if Cin % 32 or N % 32:
             raise ValueError("channel counts must be multiples of 32")
+        if b is not None and b.numel() != N:
+            raise ValueError(f"b must have {N} values, has {b.numel()}")
+        if any(t is not None and t.device != x.device for t in (w, b)):
+            raise ValueError(f"w and b must be on {x.device}")
         xb = _bits(x)
         kind = PK_CONVT if transpose else PK_PW            # 3x3 Conv2D arrives here as its ConvT equivalent
         y = _conv_fwd(xb, _pack(w, kind, ks, Cin, N), None if b is None else b.detach().float().contiguous(),

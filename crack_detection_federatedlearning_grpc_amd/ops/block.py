@@ -25,14 +25,15 @@ def self_attention2d(x: torch.Tensor, norm_weight: torch.Tensor, norm_bias: torc
     if x.dim() != 4:
         raise ValueError(f"self_attention2d: x must be (B, H, W, C), got {tuple(x.shape)}")
     kv = heads if kv_heads is None else kv_heads
-    B, H, W, _ = x.shape
+    B, H, W, C = x.shape
     total = heads + 2 * kv
-    if heads < 1 or kv < 1 or w_qkv.dim() != 4 or w_qkv.shape[3] % total:
-        raise ValueError(f"self_attention2d: w_qkv {tuple(w_qkv.shape)} does not hold {heads} query and 2 x {kv} key "
-                         f"and value heads")
+    if heads < 1 or kv < 1 or w_qkv.dim() != 4 or tuple(w_qkv.shape[:3]) != (1, 1, C) or w_qkv.shape[3] % total:
+        raise ValueError(f"self_attention2d: w_qkv {tuple(w_qkv.shape)} does not make {heads} query and 2 x {kv} key "
+                         f"and value heads of {C} channels")
     D = w_qkv.shape[3] // total
-    if D % 8 or w_out.dim() != 4 or w_out.shape[2] != heads * D:
-        raise ValueError(f"self_attention2d: w_out {tuple(w_out.shape)} does not take {heads} heads of {D} channels")
+    if D % 8 or tuple(w_out.shape) != (1, 1, heads * D, C):
+        raise ValueError(f"self_attention2d: w_out {tuple(w_out.shape)} does not take {heads} heads of {D} channels "
+                         f"to {C}")
     qkv = conv2d(layer_norm(x, norm_weight, norm_bias, eps), w_qkv, b_qkv).view(B, H * W, total, D)
     pos = grid_positions(H, W, device=x.device)
     qk = rotary(qkv[:, :, :heads + kv], pos, (D // 2, D // 2), theta)
