@@ -78,18 +78,22 @@ class _Conv(torch.autograd.Function):
             raise ValueError(f"b must have {N} values, has {b.numel()}")
         if any(t is not None and t.device != x.device for t in (w, b)):
             raise ValueError(f"w and b must be on {x.device}")
+        ctx.save_for_backward(x, w)
+        ctx.meta = (B, H, W, Cin, N, ks, transpose, b is not None)
         xb = _bits(x)
+        if x.numel() == 0:                                 # no pixel, no launch
+            return x.new_empty(B, H, W, N)
         kind = PK_CONVT if transpose else PK_PW            # 3x3 Conv2D arrives here as its ConvT equivalent
         y = _conv_fwd(xb, _pack(w, kind, ks, Cin, N), None if b is None else b.detach().float().contiguous(),
                       B, H, W, Cin, N, ks)
-        ctx.save_for_backward(x, w)
-        ctx.meta = (B, H, W, Cin, N, ks, transpose, b is not None)
         return y.view(torch.bfloat16)
 
     @staticmethod
     def backward(ctx, gy):
         x, w = ctx.saved_tensors
         B, H, W, Cin, N, ks, transpose, has_b = ctx.meta
+        if x.numel() == 0:
+            return torch.zeros_like(x), torch.zeros_like(w), gy.new_zeros(N, dtype=torch.float32) if has_b else None, None
         C = hip()
         gb = _bits(gy)
         gx = gw = gbias = None

@@ -835,7 +835,7 @@ int conv3x3_split_k(const ConvParams& p) {
   const int chunks = p.Cin / BK;
   const int below = cfl_tune(TUNE_CONV3_SPLIT_BLOCKS) > 0 ? cfl_tune(TUNE_CONV3_SPLIT_BLOCKS) : 192;
   const int target = cfl_tune(TUNE_CONV3_SPLIT_TARGET) > 0 ? cfl_tune(TUNE_CONV3_SPLIT_TARGET) : 384;
-  if (blocks >= below || chunks < 2) return 1;
+  if (blocks >= below || blocks < 1 || chunks < 2) return 1;
   int s = (target + blocks - 1) / blocks;
   if (s > chunks) s = chunks;
   const int per = (chunks + s - 1) / s;

@@ -488,7 +488,7 @@ int conv_igemm_splits(const ConvParams& p) {
   const int bm = t128 ? 128 : p.N % 64 == 0 ? 64 : 128;
   const int bn = t128 ? 128 : p.N % 64 == 0 ? 64 : 32;
   const int blocks = ((p.M + bm - 1) / bm) * (p.N / bn);
-  if (blocks >= 192 || KT < 16) return 1;
+  if (blocks >= 192 || blocks < 1 || KT < 16) return 1;
   int s = (384 + blocks - 1) / blocks;
   if (s > KT / 8) s = KT / 8;
   if (s > 16) s = 16;

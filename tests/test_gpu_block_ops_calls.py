@@ -72,3 +72,14 @@ def test_pending_signs_are_read():
     assert torch.equal(y, want)
     for s, t in zip(torch.autograd.grad(y, (w, b), one), torch.autograd.grad(want, (u, v), one.clone())):
         assert torch.equal(s, t)
+
+
+def test_block_of_an_empty_batch():
+    x = torch.zeros(0, 4, 4, 512, dtype=BF, device=DEV, requires_grad=True)
+    w = [torch.ones(512, device=DEV), torch.zeros(512, device=DEV), rnd((1, 1, 512, 12 * 128), FF, 0),
+         rnd((1, 1, 512, 512), FF, 1)]
+    w = [t.requires_grad_() for t in w]
+    y = ops.self_attention2d(x, *w, heads=4)
+    assert y.shape == x.shape
+    for g, t in zip(torch.autograd.grad(y.sum(), [x, *w]), [x, *w]):
+        assert g.shape == t.shape and not g.any()
