@@ -274,9 +274,8 @@ CFL_DEVICE float max_halves(float v) {
 // sums of many, are in it, or above 65,504 where they are not. A lane holds ds of one row (dq) or one key (dk), and its
 // sums are that row's or key's: so they carry a power of two, f = 2^ef, as a softmax carries its maximum, and are divided
 // by it when they are stored. f starts so high that any ds which counts (2^-59 and more) brings it down; from then on the
-// largest ds so far is 2^-4 to 2, and what two parts cannot hold is below 2^-21 of it. Whether one has reached 2 is a bit
-// of the packed values: 4 operations for 16 of them, and a branch that is seldom taken (16 images x 8 heads x 1,024 tokens
-// of 64 channels: dq 82 -> 88 us, dk and dv 123 -> 134).
+// largest ds so far is 2^-4 to 2, and what two parts cannot hold is below 2^-21 of it: 8 comparisons for 16 of them, and a
+// branch that is seldom taken (16 images x 8 heads x 1,024 tokens of 64 channels: dq 82 -> 84 us, dk and dv 125 -> 136).
 template <class T>
 struct Fit {
   float f, ef;
@@ -288,15 +287,11 @@ struct Fit {
   // lane's). What a lane does goes by its own values alone.
   template <bool FINE, class F>
   CFL_DEVICE void pack(f16v& x, Packed<T, FINE>* ds, const F& lower) {
-    ds[0].set(x, 0);
-    ds[1].set(x, 1);
     if constexpr (T::NARROW) {
-      const u4v a = __builtin_bit_cast(u4v, ds[0].hi), b = __builtin_bit_cast(u4v, ds[1].hi);
-      const uint32_t any = (a[0] | a[1] | a[2]) | (a[3] | b[0] | b[1]) | (b[2] | b[3]);
-      if (__any((any & 0x40004000u) != 0)) {
-        float mx = fabsf(x[0]);                            // NaN is passed over; an infinity stays one and lowers nothing
+      float mx = fabsf(x[0]);                              // NaN is passed over; an infinity stays one and lowers nothing
 #pragma unroll
-        for (int e = 1; e < 16; ++e) mx = fmaxf(mx, fabsf(x[e]));
+      for (int e = 1; e < 16; ++e) mx = fmaxf(mx, fabsf(x[e]));
+      if (__any(mx >= 2.f)) {
         mx = max_halves(mx);
         const int down = mx >= 2.f && mx < INFINITY ? -3 - __builtin_amdgcn_frexp_expf(mx) : 0;
         const float g = ldexpf(1.f, down);
@@ -305,10 +300,10 @@ struct Fit {
         lower(g);
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] *= g;
-        ds[0].set(x, 0);
-        ds[1].set(x, 1);
       }
     }
+    ds[0].set(x, 0);
+    ds[1].set(x, 1);
   }
   CFL_DEVICE float undo(float mul) const { return T::NARROW ? mul / f * p_undo<T>() : mul; }
 };
