@@ -362,17 +362,17 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
     const bf16_t* dst = smem + buf * 2 * TILE + wid * 512;
 #pragma unroll
     for (int n = 0; n < CH; ++n) {
-      const int r = r0 + vrow[n], i = fdiv(r, p.div_g), g = r - i * p.G;
-      const bool in = vrow[n] < rem && vd[n] < p.D;
+      const int r = imin(r0 + vrow[n], p.M - 1), i = fdiv(r, p.div_g), g = r - i * p.G;
+      const bool in = vd[n] < p.D;
       const uint32_t oq = (uint32_t)((i - i0) * (int)p.q.ss + g * (int)p.q.sh + vd[n]) * 2;
       const uint32_t og = (uint32_t)((i - i0) * (int)p.go.ss + g * (int)p.go.sh + vd[n]) * 2;
       dma16(rq, in ? oq : CFL_OOB, dst + NT * 8 * n);
-      dma16(rg, in ? og : CFL_OOB, dst + TILE + NT * 8 * n);
+      dma16(rg, in && vrow[n] < rem ? og : CFL_OOB, dst + TILE + NT * 8 * n);
     }
-    // rows past the last read 0 everywhere: p is finite, do = 0, ds = 0
+    // rows past the last: the last row's query and lse2 (0 times a key that is not finite would be NaN), do = delta = 0
     if (wid < 2) {
       const u4v rs = rsrc((wid ? p.delta : p.lse2) + (int64_t)bh * p.M + r0);
-      dma4(rs, lane < imin(rem, RT) ? 4u * lane : CFL_OOB, &sstat[buf][wid][0]);
+      dma4(rs, wid == 0 ? 4u * imin(lane, rem - 1) : lane < rem ? 4u * lane : CFL_OOB, &sstat[buf][wid][0]);
     }
   };
 

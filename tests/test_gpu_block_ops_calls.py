@@ -1,5 +1,7 @@
 """Calls of attention, rotary positions and layer norm that are unusual, not wrong, or that have to be refused (marked
 gpu)."""
+import math
+
 import pytest
 import torch
 
@@ -13,7 +15,7 @@ from torch.fx.experimental.proxy_tensor import make_fx  # noqa: E402
 from crack_detection_federatedlearning_grpc_amd import ops  # noqa: E402
 
 DEV = torch.device("cuda")
-BF, FF = torch.bfloat16, torch.float32
+BF, HF, FF = torch.bfloat16, torch.float16, torch.float32
 
 
 def rnd(shape, dt, seed):
@@ -83,3 +85,17 @@ def test_block_of_an_empty_batch():
     assert y.shape == x.shape
     for g, t in zip(torch.autograd.grad(y.sum(), [x, *w]), [x, *w]):
         assert g.shape == t.shape and not g.any()
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("Sq,Sk,D", [(1, 40, 32), (33, 40, 64), (100, 130, 96), (70, 300, 128)])
+def test_a_key_of_minus_infinity_gives_its_value_no_gradient(Sq, Sk, D, causal, dt):
+    """Its weight is 0 in every row, and the rows that fill up the last tile add nothing."""
+    q, k, v, go = (rnd((1, n, 2, D), dt, i) for i, n in enumerate((Sq, Sk, Sk, Sq)))
+    q[..., 0] = q[..., 0].abs() + 0.5
+    dead = torch.arange(Sk, device=DEV) % 3 == 1
+    k[:, dead, :, 0] = -math.inf
+    v.requires_grad_()
+    (dv,) = torch.autograd.grad(ops.attention(q, k, v, causal=causal), v, go)
+    assert (dv[:, dead] == 0).all() and torch.isfinite(dv).all()
