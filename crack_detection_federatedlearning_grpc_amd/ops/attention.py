@@ -29,8 +29,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optional[
       mask:    bool, True = may attend, broadcastable to (B, Hq, Sq, Sk). It is packed to bits once per call; tiles in
                which it allows nothing are skipped.
       causal:  key j for query i where j <= i + Sk - Sq (the last query attends the last key).
-    A query that may attend nothing gets 0, and no gradient comes from it. Whatever a key or value holds where it is
-    not allowed, infinities and NaN too, has no effect.
+    A query that may attend nothing gets 0, and no gradient comes from it; one whose every score is -inf gets NaN.
+    Whatever a key or value holds where it is not allowed, infinities and NaN too, has no effect.
 
     Returns (B, Sq, Hq, D); with return_lse also the fp32 (B, Hq, Sq) log of the softmax' sum (-inf where a query may
     attend nothing; it has no gradient). The backward pass computes the probabilities again; its results do not depend

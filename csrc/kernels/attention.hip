@@ -18,6 +18,7 @@
 // join = 3.2 TB/s.
 // Rows that may attend nothing are 0 and their saved lse2 is +inf (exp2(s - inf) = 0 in the backward pass).
 #include <algorithm>
+#include <cfloat>
 
 #include "attention.h"
 
@@ -31,6 +32,13 @@ constexpr float SLACK = 8.f;
 
 // up to this many rows the four waves of a block split the keys of a tile, beyond it the rows
 constexpr int FEW_ROWS = 32;
+
+// whether the mask bits of a tile's KW keys allow one of the first `left`
+template <int KW>
+CFL_DEVICE bool attended(unsigned long long bits, int left) {
+  const unsigned long long m = left >= 64 ? ~0ull : (1ull << imax(left, 0)) - 1;
+  return (bits & m & (KW == 64 ? ~0ull : (1ull << (KW & 63)) - 1)) != 0;
+}
 
 // QT: 32-row tiles per wave; WR x WK: waves along the rows and along the keys of a tile; KW keys per wave and tile
 template <class T, int DP, int QT, int WR, int WK, int KW, int MINW, int KIND, bool FINE>
@@ -223,6 +231,11 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
 #pragma unroll
             for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[k][u][e]);
           mx = max_halves(mx) * sc;
+          // a row with a key that it may attend has a maximum, if all of its scores are -inf or NaN: its sum is then not
+          // that of an empty row
+          const int left = lim[u] - key0;
+          const bool some = KIND == ATTN_PLAIN || (MASK && part ? attended<KW>(cur[u], left) : left > 0);
+          mx = fmaxf(mx, some ? -FLT_MAX : -INFINITY);
           if (__any(mx > m[u] + SLACK)) {
             // only the rows that need it: what a row rounds does not depend on the rows next to it
             const bool up = mx > m[u] + SLACK;
@@ -350,7 +363,8 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
       }
       continue;
     }
-    const float inv = l[u] == 0.f ? 0.f : 1.f / l[u];
+    const bool none = m[u] == -INFINITY;                   // l may be 0 elsewhere too: every score -inf, 0 / 0
+    const float inv = none ? 0.f : 1.f / l[u];
     const int64_t at = b * p.o.sb + ri[u] * p.o.ss + (hk * p.G + rg[u]) * p.o.sh;
     bf16_t *o = reinterpret_cast<bf16_t*>(p.o.p) + at, *rest = p.o_rest ? p.o_rest + at : nullptr;
 #pragma unroll
@@ -358,7 +372,7 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
       store_row<T>(o, acc[d][u], inv, d, p.D, h, ok, rest);
     }
     if (ok && h == 0 && p.lse2)
-      p.lse2[row] = l[u] == 0.f ? INFINITY : m[u] + __builtin_amdgcn_logf(l[u]) - (T::UP + T::P_UP);
+      p.lse2[row] = none ? INFINITY : m[u] + __builtin_amdgcn_logf(l[u]) - (T::UP + T::P_UP);
   }
 }
 
@@ -400,7 +414,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnParams p) {
   }
   const int bh = (int)(row / p.M), r = (int)(row - (int64_t)bh * p.M), b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const int i = fdiv(r, p.div_g), g = r - i * p.G;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const bool none = mn == -INFINITY;
+  const float inv = none ? 0.f : 1.f / l;
   if (d < p.D) {
     const int64_t at = b * p.o.sb + i * p.o.ss + (hk * p.G + g) * p.o.sh + d;
     a0 *= inv; a1 *= inv; a2 *= inv; a3 *= inv;
@@ -411,7 +426,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnParams p) {
           make_uint2(T::pack2((a0 - T::lo(w.x)) * T::REST, (a1 - T::hi(w.x)) * T::REST),
                      T::pack2((a2 - T::lo(w.y)) * T::REST, (a3 - T::hi(w.y)) * T::REST));
   }
-  if (d == 0 && p.lse2) p.lse2[row] = l == 0.f ? INFINITY : mn + __builtin_amdgcn_logf(l) - (T::UP + T::P_UP);
+  if (d == 0 && p.lse2) p.lse2[row] = none ? INFINITY : mn + __builtin_amdgcn_logf(l) - (T::UP + T::P_UP);
 }
 
 // mask bytes -> words: one wave per (32 mask rows, 64 keys), all of its loads under way together

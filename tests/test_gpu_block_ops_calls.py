@@ -99,3 +99,50 @@ def test_a_key_of_minus_infinity_gives_its_value_no_gradient(Sq, Sk, D, causal, 
     v.requires_grad_()
     (dv,) = torch.autograd.grad(ops.attention(q, k, v, causal=causal), v, go)
     assert (dv[:, dead] == 0).all() and torch.isfinite(dv).all()
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("kind", ["plain", "lengths", "causal", "mask", "mask causal", "bits"])
+@pytest.mark.parametrize("Sq,Sk", [(1, 90), (20, 3000), (150, 150), (300, 70), (200, 2500)])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_rows_whose_every_score_is_minus_infinity(D, Sq, Sk, kind, dt):
+    """softmax has no value there: NaN, as any broken row, and not the 0 of a row that may attend nothing. Rows with a
+    finite score are what they are without the others."""
+    B = 3
+    q, k, v, go = (rnd((B, n, 2, D), dt, i) for i, n in enumerate((Sq, Sk, Sk, Sq)))
+    q[..., 0] = q[..., 0].abs() + 0.5
+    g = torch.Generator().manual_seed(4)
+    dead = torch.rand(B, Sk, generator=g) < 0.5
+    dead[0] = True                                           # an image without a finite score
+    dead[1, :Sk // 2] = True                                 # one whose first half has none
+    dead = dead.to(DEV)
+    k[..., 0] = torch.where(dead[..., None], torch.full_like(k[..., 0], -math.inf), k[..., 0])
+    ok, kw = torch.ones(B, Sq, Sk, dtype=torch.bool, device=DEV), {}
+    if "causal" in kind:
+        ok = ok & (torch.arange(Sk, device=DEV) <= torch.arange(Sq, device=DEV)[:, None] + Sk - Sq)
+        kw["causal"] = True
+    if kind == "lengths":
+        kw["lengths"] = torch.tensor([Sk - 3, Sk // 2, 0], dtype=torch.int32, device=DEV)
+        ok = ok & (torch.arange(Sk, device=DEV) < kw["lengths"][:, None])[:, None]
+    if "mask" in kind or kind == "bits":
+        m = (torch.rand(B, Sq, Sk, generator=g) < (0.02 if kind == "bits" else 0.6)).to(DEV)
+        m[:, Sq // 2] = False
+        kw["mask"], ok = m[:, None], ok & m
+    ins = [t.detach().requires_grad_() for t in (q, k, v)]
+    out, lse = ops.attention(*ins, return_lse=True, **kw)
+    alive = ok & ~dead[:, None]
+    broken = ok.any(2) & ~alive.any(2)                       # (B, Sq)
+    empty = ~ok.any(2)
+    assert broken.any() or not ok.any()
+    assert out[broken].isnan().all() and (out[empty] == 0).all() and torch.isfinite(out[~broken]).all()
+    assert (lse.transpose(1, 2)[broken | empty] == -math.inf).all() and torch.isfinite(lse.transpose(1, 2)[~(broken | empty)]).all()
+    with torch.no_grad():
+        want, wlse = ops.attention(q, k, v, mask=alive[:, None], return_lse=True)
+    live = ~(broken | empty)
+    # the same pairs count; the tiles that are walked differ, and with them the order of fp32 sums
+    assert ((out[live].double() - want[live].double()).abs() <= torch.finfo(dt).eps * (want[live].double().abs() + 2 ** -8)).all()
+    assert (lse.transpose(1, 2)[live] - wlse.transpose(1, 2)[live]).abs().max() <= 1e-5 if live.any() else True
+    dq, dk, dv = torch.autograd.grad(out, ins, go)
+    assert dq[broken].isnan().all() and (dq[empty] == 0).all()
+    hit = (ok & broken[..., None]).any(1)                    # keys that a broken row may attend
+    assert dv[hit].isnan().all() and torch.isfinite(dv[~hit]).all()
