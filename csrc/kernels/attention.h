@@ -132,7 +132,7 @@ CFL_DEVICE s8v frag_t(const bf16_t* rows, const TransAt<DP>& t, int dt) {
 // 0 * inf and 0 * NaN are NaN: what a key holds where no query may attend it would show in every row. So after its walk
 // a block with any mask looks whether its sums are finite (they are, in all but broken calls) and if not walks again
 // with the operand's values replaced by 0 (clean), and those of pairs with a probability put back: `poison` adds +inf /
-// -inf to the sums whose pairs of p > 0 hold +inf or NaN / -inf or NaN (both: NaN).
+// -inf to the sums whose pairs of p > 0 in fp32 (the bits of `weighed`) hold +inf or NaN / -inf or NaN (both: NaN).
 template <class T>
 CFL_DEVICE s8v clean(const s8v& a, s8v& pos, s8v& neg) {
   s8v r;
@@ -147,10 +147,10 @@ CFL_DEVICE s8v clean(const s8v& a, s8v& pos, s8v& neg) {
   return r;
 }
 template <class T>
-CFL_DEVICE void poison(f16v& acc, const s8v& pos, const s8v& neg, const s8v& p) {
+CFL_DEVICE void poison(f16v& acc, const s8v& pos, const s8v& neg, uint32_t some) {
   s8v one;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) one[j] = p[j] != 0 ? T::ONE : (short)0;
+  for (int j = 0; j < 8; ++j) one[j] = some >> j & 1 ? T::ONE : (short)0;
   f16v z;
 #pragma unroll
   for (int e = 0; e < 16; ++e) z[e] = 0.f;
@@ -160,6 +160,12 @@ CFL_DEVICE void poison(f16v& acc, const s8v& pos, const s8v& neg, const s8v& p) 
   const f16v b = T::mma(neg, one, z);
 #pragma unroll
   for (int e = 0; e < 16; ++e) acc[e] -= b[e] > 0.f ? INFINITY : 0.f;
+}
+CFL_DEVICE uint32_t weighed(const f16v& p) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) r |= p[e] != 0.f ? 1u << e : 0;
+  return r;
 }
 // 0, or NaN if any element is not finite
 CFL_DEVICE float finite_sum(const f16v& v) {

@@ -223,6 +223,7 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
         }
         __builtin_amdgcn_s_setprio(0);
         Packed<T, FINE> pb[QT][2 * NK];
+        uint32_t seen[QT][NK];
 #pragma unroll
         for (int u = 0; u < QT; ++u) {
           float mx = s[0][u][0];
@@ -256,6 +257,7 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
               s[k][u][e] = exp2_(fmaf(s[k][u][e], sc, -ms));
               sum += s[k][u][e];
             }
+            if constexpr (SAFE) seen[u][k] = weighed(s[k][u]);
             pb[u][2 * k].set(s[k][u], 0);
             pb[u][2 * k + 1].set(s[k][u], 1);
           }
@@ -272,7 +274,7 @@ __global__ __launch_bounds__(64 * WR * WK, MINW) void attn_fwd_kernel(const Attn
               __builtin_amdgcn_sched_barrier(0);           // few registers matter here, not speed
               a = clean<T>(a, pos, neg);
 #pragma unroll
-              for (int u = 0; u < QT; ++u) poison<T>(acc[d][u], pos, neg, pb[u][ks].hi);
+              for (int u = 0; u < QT; ++u) poison<T>(acc[d][u], pos, neg, seen[u][ks >> 1] >> 8 * (ks & 1));
             }
 #pragma unroll
             for (int u = 0; u < QT; ++u) acc[d][u] = pb[u][ks].mma(a, acc[d][u]);

@@ -478,6 +478,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
           if (VL && kk % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         }
         Packed<T, FINE> pb[KQ][2], db[KQ][2];
+        uint32_t seen[KQ];
         if (VL) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int u = 0; u < KQ; ++u) {
@@ -501,6 +502,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[u][e] = (e & 3) + 8 * (e >> 2) >= from ? s[u][e] : 0.f;
           }
+          if constexpr (SAFE) seen[u] = weighed(s[u]);
           pb[u][0].set(s[u], 0);
           pb[u][1].set(s[u], 1);
 #pragma unroll
@@ -528,7 +530,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
                 __builtin_amdgcn_sched_barrier(0);           // few registers matter here, not speed
                 a = clean<T>(a, pos, neg);
 #pragma unroll
-                for (int u = 0; u < KQ; ++u) poison<T>(dv[d][u], pos, neg, pb[u][ks].hi);
+                for (int u = 0; u < KQ; ++u) poison<T>(dv[d][u], pos, neg, seen[u] >> 8 * ks);
               }
 #pragma unroll
               for (int u = 0; u < KQ; ++u) dv[d][u] = pb[u][ks].mma(a, dv[d][u]);

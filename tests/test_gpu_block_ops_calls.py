@@ -146,3 +146,32 @@ def test_rows_whose_every_score_is_minus_infinity(D, Sq, Sk, kind, dt):
     assert dq[broken].isnan().all() and (dq[empty] == 0).all()
     hit = (ok & broken[..., None]).any(1)                    # keys that a broken row may attend
     assert dv[hit].isnan().all() and torch.isfinite(dv[~hit]).all()
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("kind", ["causal", "mask"])
+@pytest.mark.parametrize("Sq", [20, 150])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_a_small_weight_hides_no_infinity(D, Sq, kind, dt):
+    """A weight of 2^-43 of the row's largest is none that 16 bits hold, and still not 0."""
+    S = 150
+    q, k, v, go = (rnd((1, n, 2, D), dt, i) for i, n in enumerate((Sq, S, S, Sq)))
+    q[..., 0], k[..., 0] = 8, 0
+    j = S - Sq + 5                                           # the rows from 5 on may attend it
+    k[:, j] = 0
+    k[:, j, :, 0] = -30 * math.sqrt(D) / 8
+    tri = torch.arange(S, device=DEV) <= torch.arange(Sq, device=DEV)[:, None] + S - Sq
+    kw = {"causal": True} if kind == "causal" else {"mask": tri}
+    want = ops.attention(q, k, v, **kw)
+    for x in (math.inf, -math.inf, math.nan):
+        w = v.clone()
+        w[0, j, :, 3] = x
+        out = ops.attention(q, k, w, **kw)
+        hit = out[0, 5:, :, 3].float()
+        assert (hit.isnan().all() if math.isnan(x) else (hit == x).all())
+        assert torch.equal(out[0, :5], want[0, :5])
+    g = go.clone()
+    g[0, Sq - 1, :, 4] = math.inf                            # the row that attends every key
+    v.requires_grad_()
+    (dv,) = torch.autograd.grad(ops.attention(q, k, v, **kw), v, g)
+    assert (dv[..., 4] == math.inf).all() and torch.isfinite(dv[..., :4]).all()
