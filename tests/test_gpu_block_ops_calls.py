@@ -175,3 +175,44 @@ def test_a_small_weight_hides_no_infinity(D, Sq, kind, dt):
     v.requires_grad_()
     (dv,) = torch.autograd.grad(ops.attention(q, k, v, **kw), v, g)
     assert (dv[..., 4] == math.inf).all() and torch.isfinite(dv[..., :4]).all()
+
+
+def test_calls_at_once_on_two_streams_and_threads_each_of_them():
+    """Two threads on streams of their own: every result of every call is what a call alone gives, and none raises."""
+    import threading
+    cases = []
+    for seed, shape in ((1, (1, 30, 3000, 2, 2, 64)), (7, (2, 600, 500, 2, 1, 32))):
+        B, Sq, Sk, Hq, Hkv, D = shape
+        q, k, v, go = (rnd((B, n, h, D), BF, seed + i) for i, (n, h) in enumerate(((Sq, Hq), (Sk, Hkv), (Sk, Hkv), (Sq, Hq))))
+        x, w, gy = rnd((3000, 96), BF, seed), rnd((96,), FF, seed), rnd((3000, 96), BF, seed + 1)
+        mask = (torch.rand(Sk, generator=torch.Generator().manual_seed(seed)) < 0.7)[None, None, None].to(DEV)
+        pos = torch.arange(Sq, device=DEV)[None]
+
+        def run(q=q, k=k, v=v, go=go, x=x, w=w, gy=gy, mask=mask, pos=pos, D=D):
+            ins = [t.detach().requires_grad_() for t in (q, k, v, x, w)]
+            out = [ops.attention(ops.rotary(ins[0], pos, (D,)), ins[1], ins[2], mask), ops.layer_norm(*ins[3:])]
+            return [t.detach() for t in out] + list(torch.autograd.grad(out, ins, [go, gy]))
+        cases.append((run, run()))
+    torch.cuda.synchronize()
+    bad, done, together = [], [], threading.Barrier(2, timeout=30)
+
+    def work(n, run, want):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                together.wait()
+                got = [run() for _ in range(20)]
+                s.synchronize()
+            for i, g in enumerate(got):
+                bad.extend((n, i, j) for j, (a, b) in enumerate(zip(g, want)) if not torch.equal(a, b))
+            done.append(n)
+        except Exception as e:  # noqa: BLE001 - a thread's exception would be lost
+            bad.append((n, repr(e)))
+
+    ts = [threading.Thread(target=work, args=(n, *c)) for n, c in enumerate(cases)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join(60)
+        assert not t.is_alive()
+    assert not bad and sorted(done) == [0, 1]
