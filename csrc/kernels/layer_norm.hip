@@ -73,7 +73,7 @@ CFL_DEVICE float lane_sum(float v) {
   return v;
 }
 
-// sum / n by the reciprocal, corrected once: the quotient of a sum of equal values is that value
+// sum / n by the reciprocal, corrected once: where the sum of equal values is exact, their mean is that value
 CFL_DEVICE float mean_of(float sum, float n, float inv) {
   const float m = sum * inv;
   return fmaf(fmaf(-m, n, sum), inv, m);
@@ -282,8 +282,8 @@ __global__ __launch_bounds__(NT) void ln_bwd_kernel(const LayerNormParams p) {
         s1 += red2[par][gr][u].y;
       }
     }
-    // the mean taken from dy w before anything is scaled: a row of one column, or of equal ones, gives 0 and not the
-    // rounding of a product
+    // the mean taken from dy w before anything is scaled: a row of one column gives 0 and not the rounding of a product
+    // (equal values in several columns leave the rounding of their sum and of 1 / C)
     const float m0 = s0 * sh.inv, m1 = s1 * sh.inv;
     E* yr = reinterpret_cast<E*>(p.y) + r * p.C;
 #pragma unroll
