@@ -10,6 +10,7 @@ pytestmark = pytest.mark.gpu
 if not torch.cuda.is_available():
     pytest.skip("no GPU", allow_module_level=True)
 
+import torch.utils.checkpoint  # noqa: E402
 from torch.fx.experimental.proxy_tensor import make_fx  # noqa: E402
 
 from crack_detection_federatedlearning_grpc_amd import ops  # noqa: E402
@@ -216,3 +217,44 @@ def test_calls_at_once_on_two_streams_and_threads_each_of_them():
         t.join(60)
         assert not t.is_alive()
     assert not bad and sorted(done) == [0, 1]
+
+
+def test_inference_mode_and_saved_tensor_hooks(call):
+    """What autograd saves may come back from elsewhere, as a copy with other strides; without autograd nothing is."""
+    f, x = call
+    x.requires_grad_()
+    y = f(x)
+    go = torch.ones_like(y)
+    (want,) = torch.autograd.grad(y, x, go)
+    with torch.inference_mode():
+        assert torch.equal(f(x.detach().clone()), y)
+    with torch.autograd.graph.save_on_cpu():
+        z = f(x)
+    assert torch.equal(torch.autograd.grad(z, x, go)[0], want)
+    z = torch.utils.checkpoint.checkpoint(f, x, use_reentrant=False)
+    assert torch.equal(torch.autograd.grad(z, x, go)[0], want)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_saved_slices_come_back_as_copies(causal):
+    """q, k and v are slices of one tensor, with a mask and lengths, and what is saved of them returns contiguous."""
+    qkv = rnd((2, 70, 8, 64), BF, 0)
+    q, k, v = (t.detach().requires_grad_() for t in qkv.split([4, 2, 2], 2))
+    assert not q.is_contiguous()
+    mask = (torch.rand(2, 1, 70, 70, generator=torch.Generator().manual_seed(1)) < 0.6).to(DEV)
+    lengths = torch.tensor([[70, 0], [33, 0]], dtype=torch.int32, device=DEV)[:, 0]
+    go = rnd((2, 70, 4, 64), BF, 1)
+    want = torch.autograd.grad(ops.attention(q, k, v, mask, lengths, causal), (q, k, v), go)
+    with torch.autograd.graph.save_on_cpu():
+        out = ops.attention(q, k, v, mask, lengths, causal)
+    for a, b in zip(torch.autograd.grad(out, (q, k, v), go), want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("dt", [BF, HF, FF])
+def test_rotary_of_an_odd_number_of_channels(dt, inter):
+    x, pos = rnd((2, 9, 3, 33), dt, 0), torch.arange(18, device=DEV).view(2, 9)
+    whole = ops.rotary(x, pos, (16, 16), interleaved=inter)
+    assert torch.equal(whole[..., 32:], x[..., 32:])
+    assert torch.equal(whole[..., :32], ops.rotary(x[..., :32], pos, (16, 16), interleaved=inter))
