@@ -10,13 +10,13 @@
 // Split. Four waves own 32 rows each and share the tiles (64 keys); up to 32 rows in all, the waves split a tile's keys
 // instead and join through LDS. Few row blocks: blocks share a walk (attn_splits) and a second launch joins the parts.
 // 256 registers, two waves a SIMD or more: at 512 the compiler puts the first product's result into accumulation
-// registers and copies every score (16 heads x 4,096 tokens x 128 channels: 479 us against 294).
-// Bound. Up to 64 channels by the vector unit (75 % busy; 32 scores cost a lane 32 exponentials of 8 cycles and 128 other
-// operations, the products half of that time), at 128 channels by both it and the matrix cores; no LDS bank conflicts.
-// 2 images x 16 heads x 4,096 tokens: 128 channels 283 us = 972 TFLOP/s; 4 images, 64 channels 314 us = 875 (a library
-// product of 8,192^3 reaches 1,213). One query of 64 (image, head)s over 4,096 keys of 32 channels: 8.3 us + 2.3 us to
-// join = 3.2 TB/s.
-// Rows that may attend nothing are 0 and their saved lse2 is +inf (exp2(s - inf) = 0 in the backward pass).
+// registers and copies every score (16 heads x 4,096 tokens x 128 channels, weights in one part: 479 us against 294).
+// Bound. Up to 64 channels by the vector unit (80 % busy, the matrix cores 52 %), at 128 channels by the matrix cores
+// (58 %) and it (49 %); no LDS bank conflicts. 2 images x 16 heads x 4,096 tokens of 128 channels 376 us = 1,097 TFLOP/s
+// over the three products that two-part weights make of two; 4 images, 64 channels 420 us = 982 (a library product of
+// 8,192^3 reaches 1,213). One query of 64 (image, head)s over 4,096 keys of 32 channels: 9.0 us + 2.5 us to join = 2.9 TB/s.
+// Rows that may attend nothing are those without a maximum: 0, and their saved lse2 is +inf (exp2(s - inf) = 0 in the
+// backward pass).
 #include <algorithm>
 #include <cfloat>
 
@@ -506,7 +506,7 @@ bool attn_fine() { return cfl_tune(TUNE_ATTN_FINE) != 1; }
 
 // Blocks that share the keys of a row block: enough for two blocks a CU where there are few row blocks, at least four
 // tiles each. (Blocks of 64 rows with two waves along the keys instead, for such grids, were slower: 4 images x 8 heads
-// x 1,600 tokens of 64 channels 43 us against 40.)
+// x 1,600 tokens of 64 channels 43 us against 40, weights in one part.)
 int attn_splits(int B, int Hkv, int M, int Sk) {
   const int64_t blocks = (int64_t)((M + 127) / 128) * B * Hkv;
   const int tile = M <= FEW_ROWS ? 128 : 64;

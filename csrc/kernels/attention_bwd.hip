@@ -2,13 +2,14 @@
 //   delta_i = do_i.o_i     dp_ij = do_i.v_j     ds_ij = p_ij (dp_ij - delta_i)
 //   dv_j = sum_i p_ij do_i     dk_j = scale sum_i ds_ij q_i     dq_i = scale sum_j ds_ij k_j
 // Two kernels: one owns rows and walks the keys (delta, dq), one owns keys and walks the rows (dk, dv; the rows of every
-// head that shares the key head, so their sum needs no join). The scores and dp are computed in both: 7 products
-// instead of the 5 of a single pass, and in exchange no gradient is summed by atomics: results do not depend on the
-// order in which blocks run, and nothing but the gradients is written.
-// Bound: the matrix cores and the vector unit about equally (16 heads x 4,096 tokens of 64 channels, dk and dv: 55 % and
-// 49 % busy); the LDS carries a fragment per product, 8 of 32 cycles, without conflicts. Two images of 128 channels: 868
-// us = 1,108 TFLOP/s over the 7 products (a library product of 8,192^3: 1,213). 64 keys a wave halve the LDS traffic but
-// leave one wave a SIMD: slower at every width but 32 (128 channels 1,045 us against 953 then).
+// head that shares the key head, so their sum needs no join). The scores and dp are computed in both, and no gradient is
+// summed by atomics in exchange: results do not depend on the order in which blocks run, and nothing but the gradients is
+// written.
+// Bound: the matrix cores and the vector unit (4 images x 16 heads x 4,096 tokens of 64 channels: 65 % and 69 % busy in dq,
+// 54 % and 60 % in dk and dv; at 128 channels 65 % and 47 %, 69 % and 50 %); the LDS carries a fragment per product, 8 of 32
+// cycles, without conflicts. Two images of 128 channels: 457 + 657 us = 1,233 TFLOP/s over the 10 products that two-part
+// operands make of 7 (a library product of 8,192^3: 1,213). 64 keys a wave halve the LDS traffic but leave one wave a
+// SIMD: slower at every width but 32 (128 channels, one part: 1,045 us against 953 then).
 // delta is taken from the output before its rounding (o + what that took away): with few keys dp - delta cancels, and a
 // rounded o would leave its whole step there.
 // Rounding: P and dS enter the second products in two parts of the inputs' type (attn_fine), in fp16 times powers of two
@@ -651,9 +652,9 @@ void bwd_d(const AttnParams& p, hipStream_t st) {
 
 // Blocks that share a row block's keys (dq) and a key block's rows (dk, dv): as attn_splits, up to two blocks a CU, or
 // four for causal dk, dv, whose blocks are as unequal as their keys (2 images, 16 heads that share 2, 8,192 tokens, 128
-// channels: 2,862 / 2,041 / 2,053 us for 512 / 1,024 / 2,048 blocks); at least four tiles each. Lengths make blocks empty,
-// not unequal: more than one round of them only costs parts (6 images of 1,531 keys, all full: 122 us for 512, 131 for
-// 1,024; 60 % full: 110 and 106).
+// channels: 2,862 / 2,041 / 2,053 us for 512 / 1,024 / 2,048 blocks); at least four tiles each. Lengths make blocks
+// empty, not unequal: more than one round of them only costs parts (6 images of 1,531 keys, all full: 122 us for 512, 131
+// for 1,024; 60 % full: 110 and 106). These with operands in one part.
 void attn_bwd_splits(int B, int Hkv, int M, int Sk, bool causal, int& splits, int& kv_splits) {
   const int64_t bhn = (int64_t)B * Hkv, qb = (M + 127) / 128 * bhn, kb = std::max<int64_t>(1, (Sk + 127) / 128 * bhn);
   splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / qb, (Sk + 63) / 64 / 4));
