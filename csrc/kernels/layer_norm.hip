@@ -5,8 +5,8 @@
 // wave, a wave, or a block), so the variance is the two-pass one - sums of squares of x - mu, exact where the mean is
 // large - at no extra read. The backward pass computes mu and r again from the row it holds anyway instead of reading
 // 8 saved bytes per row (a quarter of a 32-channel bf16 row).
-// 16,384 x 4,096 fp16: forward 46 us = 5.8 TB/s, backward 93 + 5 us = 4.1 TB/s (a copy of 4 GB: 4.7; part of these
-// tensors stays in the last-level cache); 262,144 x 32 bf16: 7.8 us and 13 + 2.4 us = 4.3 and 3.3 TB/s.
+// 16,384 x 4,096 fp16: forward 47 us = 5.7 TB/s, backward 95 + 5 us = 4.0 TB/s (a copy of 4 GB: 4.7; part of these
+// tensors stays in the last-level cache); 262,144 x 32 bf16: 8.0 us and 13.6 + 3.8 us = 4.2 and 2.9 TB/s.
 // dw / db: a lane owns the same columns in every row of its block, adds them up in fp32 registers, the block joins its
 // lanes through LDS and writes one partial row; a second launch adds the partial rows in order. No atomics: results
 // do not depend on the order in which blocks run.
