@@ -128,6 +128,16 @@ CFL_DEVICE s8v frag_t(const bf16_t* rows, const TransAt<DP>& t, int dt) {
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+// the same from the first channel tile's addresses: two registers where the second walk has no more
+template <int DP>
+CFL_DEVICE s8v frag_t2(const bf16_t* rows, const TransAt<DP>& t, int dt) {
+  int x = t.at[0][0], y = t.at[0][1];
+  asm volatile("" : "+v"(x), "+v"(y));                     // not formed ahead of the loop, for all tiles at once
+  const int d = 32 * dt;
+  const s4v a = tr4(rows + (DP % 64 == 0 ? x ^ d : x + d)), b = tr4(rows + (DP % 64 == 0 ? y ^ d : y + d));
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
 // Values that are not finite, where pairs are not allowed. A product over token rows gives such a pair the factor 0, but
 // 0 * inf and 0 * NaN are NaN: what a key holds where no query may attend it would show in every row. So after its walk
 // a block with any mask looks whether its sums are finite (they are, in all but broken calls) and if not walks again

@@ -309,24 +309,24 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
   const int off = causal ? p.Sk - p.Sq : 0;
   const int wkey0 = kb * BK + wid * KQ * 32;
 
+  // B operands of the wave's own keys or values
+  auto own_frag = [&](const AttnTensor& x, int key, int kk) {
+    const int d = 16 * kk + 8 * h;
+    u4v w = {0, 0, 0, 0};
+    if (key < len && d < p.D)
+      w = *reinterpret_cast<const u4v*>(reinterpret_cast<const bf16_t*>(x.p) + b * x.sb + key * x.ss + hk * x.sh + d);
+    return __builtin_bit_cast(s8v, w);
+  };
   s8v kf[KQ][NKK], vf[KQ][VL ? 1 : NKK];
   int rmin[KQ];                                              // first row that may attend this lane's key
 #pragma unroll
   for (int t = 0; t < KQ; ++t) {
     const int key = wkey0 + 32 * t + c;
     rmin[t] = causal ? imin(imax(key - off, 0), p.Sq) * p.G : 0;
-    const bf16_t* k = reinterpret_cast<const bf16_t*>(p.k.p) + b * p.k.sb + key * p.k.ss + hk * p.k.sh;
-    const bf16_t* v = reinterpret_cast<const bf16_t*>(p.v.p) + b * p.v.sb + key * p.v.ss + hk * p.v.sh;
 #pragma unroll
     for (int kk = 0; kk < NKK; ++kk) {
-      const int d = 16 * kk + 8 * h;
-      u4v wk = {0, 0, 0, 0}, wv = wk;
-      if (key < len && d < p.D) {
-        wk = *reinterpret_cast<const u4v*>(k + d);
-        if (!VL) wv = *reinterpret_cast<const u4v*>(v + d);
-      }
-      kf[t][kk] = __builtin_bit_cast(s8v, wk);
-      if (!VL) vf[t][VL ? 0 : kk] = __builtin_bit_cast(s8v, wv);
+      kf[t][kk] = own_frag(p.k, key, kk);
+      if (!VL) vf[t][VL ? 0 : kk] = own_frag(p.v, key, kk);
     }
   }
   const bf16_t* svals = smem + 4 * TILE + wid * KQ * 32 * DP;
@@ -467,7 +467,9 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
         for (int kk = 0; kk < NKK; ++kk) {
           const s8v a = frag_x<DP>(sq + 32 * n * DP, fo, kk);
 #pragma unroll
-          for (int u = 0; u < KQ; ++u) s[u] = T::mma(a, kf[u][kk], s[u]);
+          for (int u = 0; u < KQ; ++u)
+            // the second walk reads its keys each time: it needs their registers, not speed
+            s[u] = T::mma(a, VL && SAFE ? own_frag(p.k, wkey0 + 32 * u + c, kk) : kf[u][kk], s[u]);
           if (VL && kk % 8 == 7) __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
@@ -525,7 +527,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
           for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
-              s8v a = frag_t<DP>(sg + (32 * n + 16 * ks) * DP, ta, d);
+              const bf16_t* rows = sg + (32 * n + 16 * ks) * DP;
+              s8v a = SAFE ? frag_t2<DP>(rows, ta, d) : frag_t<DP>(rows, ta, d);
               if constexpr (SAFE) {
                 s8v pos, neg;
                 __builtin_amdgcn_sched_barrier(0);           // few registers matter here, not speed
@@ -542,7 +545,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
           for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
-              s8v a = frag_t<DP>(sq + (32 * n + 16 * ks) * DP, ta, d);
+              const bf16_t* rows = sq + (32 * n + 16 * ks) * DP;
+              s8v a = SAFE ? frag_t2<DP>(rows, ta, d) : frag_t<DP>(rows, ta, d);
               if constexpr (SAFE) {                            // an allowed query that is not finite shows in its scores
                 s8v pos, neg;
                 __builtin_amdgcn_sched_barrier(0);           // few registers matter here, not speed

@@ -5,8 +5,9 @@
 // backward pass is the same turn by the negative angle.
 // Memory bound: x is read once, y written once (2 x 16,368 tokens x 20 heads x 128 channels bf16: 65 to 72 us = 5.1 to
 // 4.7 TB/s; a copy of 4 GB: 4.7; 256 tokens x 16 heads x 32: 4.7 us, half of it the launch). An angle is computed once per
-// token and pair and used for all heads a thread walks. It is formed in revolutions in 64 bits (a position of 2^30 leaves 22 bits behind the point, fp32 would
-// leave none), reduced to an eighth of a turn there, and only the rest is rounded to fp32.
+// token and pair and used for all heads a thread walks. It is formed in revolutions in 64 bits (a position of 2^30 leaves
+// 22 bits behind the point, fp32 would leave none), reduced to an eighth of a turn there, and only the rest is rounded to
+// fp32.
 #include <algorithm>
 
 #include "common.h"
