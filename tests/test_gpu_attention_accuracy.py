@@ -2,9 +2,11 @@
 values (marked gpu).
 
 The measure is the 2-norm of an output's error over that of the 64-bit result rounded to the tensors' type. 1 is an
-output whose only error is its own rounding. What two 16-bit parts of a weight leave is below 2^-7 of one part's
-rounding, fp32 scores and sums of these sizes are off by less than 2^-17 relative, a tenth of that at most: LIMIT. A weight
-rounded to one part alone would give sqrt(2)."""
+output whose only error is its own rounding, u = finfo.eps / 2 relative. Two 16-bit parts of a weight leave u^2 of it, at
+most 2^-8 of u. A score is a sum of D fp32 products: their roundings are independent, so that it is off by about
+sqrt(D + 4) 2^-24 of the magnitude of its terms, here below 2^-17, 2^-6 of float16's u; dp and the sums over keys or rows
+likewise. Each of these adds to 1 in squares, by less than a hundredth: LIMIT leaves ten. A weight rounded to one part
+alone would give sqrt(2)."""
 import math
 
 import pytest
