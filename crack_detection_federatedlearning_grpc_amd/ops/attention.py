@@ -30,7 +30,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optional[
                which it allows nothing are skipped.
       causal:  key j for query i where j <= i + Sk - Sq (the last query attends the last key).
     A query that may attend nothing gets 0, and no gradient comes from it; one whose every score is -inf gets NaN.
-    Whatever a key or value holds where it is not allowed, infinities and NaN too, has no effect.
+    Whatever a key or value holds where it is not allowed, infinities and NaN too, has no effect; an infinite value
+    that may be attended shows as an infinity or NaN.
 
     Returns (B, Sq, Hq, D); with return_lse also the fp32 (B, Hq, Sq) log of the softmax' sum (-inf where a query may
     attend nothing; it has no gradient). The backward pass computes the probabilities again; its results do not depend
