@@ -263,6 +263,8 @@ void backward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, con
   p.o = view(out);
   p.o_rest = reinterpret_cast<bf16_t*>(sv.rest.data_ptr());
   p.go = view(go);
+  // a softmax over one key is 1 whatever the score: no gradient, and not what the roundings of dp - delta leave
+  p.grad_scale = s.Sk == 1 ? 0.f : p.scale;
   if (dq.defined()) p.dq = view(dq);
   if (dk.defined()) p.dk = view(dk);
   if (dv.defined()) p.dv = view(dv);

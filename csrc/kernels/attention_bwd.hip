@@ -277,12 +277,12 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
     if (p.splits > 1) {
       const int64_t part = ((int64_t)sp * bhn + bh) * p.M + rb * BR + (wid * QT + u) * 32 + c;
 #pragma unroll
-      for (int d = 0; d < ND; ++d) store_part<DP>(p.ws_o + part * DP, acc[d][u], fit[u].undo(p.scale), d, h, ok);
+      for (int d = 0; d < ND; ++d) store_part<DP>(p.ws_o + part * DP, acc[d][u], fit[u].undo(p.grad_scale), d, h, ok);
       continue;
     }
     bf16_t* o = reinterpret_cast<bf16_t*>(p.dq.p) + b * p.dq.sb + ri[u] * p.dq.ss + (hk * p.G + rg[u]) * p.dq.sh;
 #pragma unroll
-    for (int d = 0; d < ND; ++d) store_row<T>(o, acc[d][u], fit[u].undo(p.scale), d, p.D, h, ok);
+    for (int d = 0; d < ND; ++d) store_row<T>(o, acc[d][u], fit[u].undo(p.grad_scale), d, p.D, h, ok);
   }
 }
 
@@ -589,14 +589,14 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
       const int64_t part = ((int64_t)sp * bhn + bh) * p.Sk + key, half = (int64_t)p.kv_splits * bhn * p.Sk;
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        store_part<DP>(p.ws_kv + part * DP, dk[d][u], fit[u].undo(p.scale), d, h, key < len);
+        store_part<DP>(p.ws_kv + part * DP, dk[d][u], fit[u].undo(p.grad_scale), d, h, key < len);
         store_part<DP>(p.ws_kv + (half + part) * DP, dv[d][u], p_undo<T>(), d, h, key < len);
       }
       continue;
     }
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
-      if (p.dk.p) store_row<T>(ko, dk[d][u], fit[u].undo(p.scale), d, p.D, h, key < p.Sk, nullptr, key >= len);
+      if (p.dk.p) store_row<T>(ko, dk[d][u], fit[u].undo(p.grad_scale), d, p.D, h, key < p.Sk, nullptr, key >= len);
       if (p.dv.p) store_row<T>(vo, dv[d][u], p_undo<T>(), d, p.D, h, key < p.Sk, nullptr, key >= len);
     }
   }

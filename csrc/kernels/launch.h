@@ -651,6 +651,7 @@ struct AttnParams {
   int fp16;
   int uneven;                       // blocks differ in work between (image, head)s: attention.h locate()
   float scale;
+  float grad_scale;                 // backward: what dq and dk are multiplied by, scale, or 0 where there is one key
   FastDiv div_g;
   int splits;                       // blocks that share the keys of a row block (forward, dq); their parts are in
   float* ws_o;                      // [splits][B][Hkv][M][DP], DP = D in whole 32s

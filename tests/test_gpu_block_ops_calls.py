@@ -258,3 +258,27 @@ def test_rotary_of_an_odd_number_of_channels(dt, inter):
     whole = ops.rotary(x, pos, (16, 16), interleaved=inter)
     assert torch.equal(whole[..., 32:], x[..., 32:])
     assert torch.equal(whole[..., :32], ops.rotary(x[..., :32], pos, (16, 16), interleaved=inter))
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("kind", ["plain", "causal", "lengths", "mask"])
+@pytest.mark.parametrize("B,Sq,Hq,Hkv,D", [(1, 1, 3, 3, 64), (4, 1, 16, 4, 16), (3, 200, 2, 1, 128)])
+def test_one_key_has_no_gradient_through_its_score(B, Sq, Hq, Hkv, D, kind, dt):
+    """A softmax over one key is 1: dq and dk are 0, dv the sum of the gradients of the rows that attend it."""
+    q, k, v, go = (rnd((B, n, h, D), dt, i) for i, (n, h) in enumerate(((Sq, Hq), (1, Hkv), (1, Hkv), (Sq, Hq))))
+    kw = {"causal": {"causal": True}, "mask": {"mask": (torch.arange(Sq, device=DEV) % 3 != 1)[:, None]},
+          "lengths": {"lengths": torch.tensor([1, 0, 1, 1][:B], dtype=torch.int32, device=DEV)}}.get(kind, {})
+    ins = [t.requires_grad_() for t in (q, k, v)]
+    dq, dk, dv = torch.autograd.grad(ops.attention(*ins, **kw), ins, go)
+    assert not dq.any() and not dk.any()
+    on = torch.ones(B, Sq, dtype=torch.bool, device=DEV)
+    if kind == "causal":
+        on[:, :-1] = False
+    elif kind == "lengths":
+        on = on & (kw["lengths"] > 0)[:, None]
+    elif kind == "mask":
+        on = on & kw["mask"].T
+    want = (go.double() * on[..., None, None]).unflatten(2, (Hkv, Hq // Hkv)).sum(3).sum(1, keepdim=True)
+    mag = (go.double().abs() * on[..., None, None]).unflatten(2, (Hkv, Hq // Hkv)).sum(3).sum(1, keepdim=True)
+    # one rounding of the result, and as many of fp32 as there are terms (a weight is 1 within two steps of fp32)
+    assert ((dv.double() - want).abs() <= torch.finfo(dt).eps / 2 * want.abs() * 1.001 + (Sq * Hq + 8) * 2.0 ** -24 * mag).all()
